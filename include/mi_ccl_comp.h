@@ -221,6 +221,113 @@ int mi_ccl_fusion_reduce_static(const size_t* counts, size_t k, int dtype, size_
                                 const void* const* own_tensors, const void* const* peers, int n_peers,
                                 void* const* out_tensors, int lp_mode, int bf16_impl, int fp16_impl, void* stream);
 
+/* ---- optimizer step on a fused group -------------------------------------------------------------- */
+
+/* What follows the reduce of a fused group's gradients, on the plan of that group (its dtype is the gradients': FLOAT32,
+ * FLOAT16 or BFLOAT16).  None of it has a counterpart in the reference.  In every call the gradients are either `grads`, a
+ * HOST array of k device pointers, one per tensor, or `fusion_buf`, a fusion buffer in the plan's layout (the reduced
+ * buffer itself, without an unpack); the other argument is NULL. */
+
+/* result[0] = |multiplier| * sqrt(sum of the squares of all gradients), result[1] = the factor that a clipped step
+ * multiplies its gradients with: multiplier * min(1, max_norm / (result[0] + 1e-6)), or multiplier when max_norm <= 0.
+ * multiplier: what the gradients are yet to be multiplied with (1 / peers after a sum, 1 / loss scale).  A norm that is not
+ * finite (squares are fp32: an element from 1.8e19 up overflows) gives result[1] = NaN, which mi_ccl_fusion_adamw takes as
+ * "no step".  result: two floats on the device.  workspace: mi_ccl_fusion_norm_workspace bytes of device memory, 8-byte
+ * aligned, needed by this call alone (calls that may overlap take one each).  The sum has a fixed order: the same
+ * gradients give the same bits. */
+size_t mi_ccl_fusion_norm_workspace(const mi_ccl_fusion_plan* plan);
+int mi_ccl_fusion_norm(mi_ccl_fusion_plan* plan, const void* const* grads, const void* fusion_buf, double multiplier,
+                       double max_norm, float* result, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Formats of the AdamW states.  Both live in the plan's layout: element i of tensor t at
+ * mi_ccl_fusion_plan_offset(t) / element size of a gradient + i, mi_ccl_fusion_plan_elements in all; between the tensors
+ * nothing is read or written.
+ *   MI_CCL_STATE_FP32  floats
+ *   MI_CCL_STATE_8BIT  bytes; 256 consecutive elements of a tensor share a power of two per state.  Needs a layout whose
+ *                      tensors start on multiples of 256 elements (align = 256 * element size).  exp_avg: a sign, 4 bits of
+ *                      exponent, 3 of mantissa (e4m3, largest 448); exp_avg_sq: 4 bits of exponent, 4 of mantissa, no sign
+ *                      (code c < 16 is c, others (16 + c % 16) * 2^(c / 16 - 1); 255 is NaN).  scales: two bytes per block of
+ *                      the layout (exp_avg's, exp_avg_sq's), 2 * ceil(elements / 256) in all; a code's value is multiplied
+ *                      with 2^(byte - 127).  An exp_avg_sq above zero is never rounded to zero.  A fresh state is all zeros:
+ *                      zero codes with zero scale bytes. */
+enum mi_ccl_state_format { MI_CCL_STATE_FP32 = 0, MI_CCL_STATE_8BIT = 1 };
+#define MI_CCL_STATE_BLOCK 256
+size_t mi_ccl_fusion_plan_elements(const mi_ccl_fusion_plan* plan);
+
+typedef struct mi_ccl_adamw_options {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;               /* this step's number, from 1 */
+    uint64_t seed;              /* of the random bits of stochastic rounding, together with the step's number */
+    int stochastic;             /* 8-bit states: 0 = rounded to nearest, 1 = up with the probability of what is cut off */
+    const int64_t* step_ptr;    /* device, or NULL: read in place of `step` (a step captured into a graph) */
+    const float* lr_ptr;        /* device, or NULL: read in place of `lr` */
+    const float* grad_scale;    /* device, or NULL for 1: every gradient is multiplied with it; not finite = no step */
+} mi_ccl_adamw_options;
+
+/* One AdamW step (decoupled weight decay) over all tensors of the plan: with g = grad_scale * gradient,
+ *   exp_avg    = beta1 * exp_avg + (1 - beta1) * g
+ *   exp_avg_sq = beta2 * exp_avg_sq + (1 - beta2) * g * g
+ *   w = w * (1 - lr * weight_decay) - lr / (1 - beta1^step) * exp_avg / (sqrt(exp_avg_sq) / sqrt(1 - beta2^step) + eps)
+ * in fp32; 8-bit states are rounded after the weights have taken the exact ones.  params: HOST array of k device pointers
+ * of param_dtype (FLOAT32, FLOAT16, BFLOAT16).  master: NULL, or for 16-bit weights the fp32 copy (in the plan's layout)
+ * that is stepped in their place; the weights are then its rounding (to nearest even).  A grad_scale that is not finite
+ * leaves weights and states as they are.  Tensors that are parameters twice must be one tensor of the plan.  Parameter
+ * groups with hyperparameters of their own take plans of their own. */
+int mi_ccl_fusion_adamw(mi_ccl_fusion_plan* plan, int param_dtype, void* const* params, const void* const* grads,
+                        const void* fusion_buf, int state_format, void* exp_avg, void* exp_avg_sq, void* scales, float* master,
+                        const mi_ccl_adamw_options* options, void* stream);
+
+/* 8-bit states to values and back (a checkpoint, a change of format); values: FLOAT32 or BFLOAT16 arrays in the plan's
+ * layout.  Decoding is exact in either type (bfloat16: from 2^-126 up).  Encoding rounds to nearest; what is not finite, and an
+ * exp_avg_sq below zero, becomes NaN. */
+int mi_ccl_fusion_state_decode(mi_ccl_fusion_plan* plan, const void* exp_avg, const void* exp_avg_sq, const void* scales,
+                               int value_dtype, void* values_avg, void* values_sq, void* stream);
+int mi_ccl_fusion_state_encode(mi_ccl_fusion_plan* plan, int value_dtype, const void* values_avg, const void* values_sq,
+                               void* exp_avg, void* exp_avg_sq, void* scales, void* stream);
+
+/* ---- tokens sorted by expert, and back ------------------------------------------------------------- */
+
+/* The local halves of an expert-parallel exchange (an all-to-all's send buffer in front of it, the weighted sum of the rows
+ * that came back behind it) and their gradients.  No counterpart in the reference.
+ *
+ * n_tokens x top_k entries carry an expert id each; an id outside [0, n_experts) is no entry (a masked token).  The sorted
+ * buffer holds expert after expert, each one's entries in the order of the tokens (and of a token's choices), each
+ * expert's rows padded to a multiple of `align` (1 = tight).  capacity > 0: an expert keeps its first `capacity` entries,
+ * the others are dropped.  n_experts <= 1024; entries and rows < 2^31.  Rows are `hidden` elements of FLOAT32, FLOAT16 or
+ * BFLOAT16, `ld` elements apart (ld >= hidden), at any element-aligned address. */
+
+/* Most rows that the sorted buffer can take: min(entries, capacity * n_experts) + padding.  Host arithmetic only. */
+int mi_ccl_token_rows(size_t n_tokens, int top_k, int n_experts, size_t align, size_t capacity, size_t* rows);
+
+/* expert_ids: n_tokens x top_k ids, INT32 or INT64 (index_dtype).  Writes positions[n_tokens x top_k], the row of each
+ * entry in the sorted buffer or -1; counts[n_experts], the entries that each expert keeps; offsets[n_experts + 1], the first
+ * row of each expert and the end of the last.  workspace: mi_ccl_token_sort_workspace bytes (0 for up to 8,192 entries),
+ * needed by this call alone.  With n_tokens == 0 counts and offsets become zero. */
+int mi_ccl_token_sort_workspace(size_t n_tokens, int top_k, int n_experts, size_t* bytes);
+int mi_ccl_token_sort(int index_dtype, const void* expert_ids, size_t n_tokens, int top_k, int n_experts, size_t align,
+                      size_t capacity, int32_t* positions, int32_t* counts, int32_t* offsets, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* out[positions[t][j]] = x[t] for every entry that has a row; rows of padding become zero, rows from offsets[n_experts] on
+ * stay as they are.  A position outside [0, out_rows) is taken as -1, here and below. */
+int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens, int top_k, size_t hidden,
+                          const int32_t* positions, const int32_t* counts, const int32_t* offsets, int n_experts, void* out,
+                          size_t ld_out, size_t out_rows, void* stream);
+
+/* out[t] = sum over j of weights[t][j] * y[positions[t][j]], accumulated in fp32 in the order of j and rounded once; a token
+ * without rows gives zeros.  weights: fp32, n_tokens x top_k, or NULL for ones -- which makes it the gradient of dispatch:
+ * x's gradient from that of the rows.  out must not overlap y. */
+int mi_ccl_token_combine(int dtype, const void* y, size_t ld_y, size_t y_rows, const int32_t* positions, const float* weights,
+                         size_t n_tokens, int top_k, size_t hidden, void* out, size_t ld_out, void* stream);
+
+/* The gradient of combine: grad_y[positions[t][j]] = weights[t][j] * grad_out[t] (rounded once; rows of padding zero, rows
+ * behind the last left as they are) and, unless grad_weights is NULL, grad_weights[t][j] = the dot product of grad_out[t]
+ * and y[positions[t][j]] in fp32, 0 where there is no row.  y may be NULL when grad_weights is.  grad_y has y_rows rows. */
+int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_grad, const void* y, size_t ld_y, size_t y_rows,
+                                  const int32_t* positions, const float* weights, const int32_t* counts,
+                                  const int32_t* offsets, int n_experts, size_t n_tokens, int top_k, size_t hidden, void* grad_y,
+                                  size_t ld_grad_y, float* grad_weights, void* stream);
+
 /* ---- measurement aid ------------------------------------------------------------------------------ */
 
 /* Read-only and write-only streams in the access shapes of the kernels above, for putting a measured ceiling of the

@@ -33,8 +33,23 @@ EXPORTS = [
     "mi_ccl_fusion_plan_create", "mi_ccl_fusion_plan_destroy", "mi_ccl_fusion_plan_bytes",
     "mi_ccl_fusion_plan_offset", "mi_ccl_fusion_pack", "mi_ccl_fusion_unpack", "mi_ccl_fusion_reduce",
     "mi_ccl_fusion_reduce_static",
+    "mi_ccl_fusion_plan_elements", "mi_ccl_fusion_norm_workspace", "mi_ccl_fusion_norm", "mi_ccl_fusion_adamw",
+    "mi_ccl_fusion_state_decode", "mi_ccl_fusion_state_encode",
+    "mi_ccl_token_rows", "mi_ccl_token_sort_workspace", "mi_ccl_token_sort", "mi_ccl_token_dispatch", "mi_ccl_token_combine",
+    "mi_ccl_token_combine_backward",
     "mi_ccl_probe_bandwidth", "mi_ccl_last_kernel", "mi_ccl_set_param", "mi_ccl_get_param",
 ]
+
+
+STATE_FP32, STATE_8BIT = 0, 1          # formats of the AdamW states
+STATE_BLOCK = 256                      # elements that share a scale in the 8-bit format
+
+
+class AdamwOptions(C.Structure):
+    """mi_ccl_adamw_options"""
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("step", C.c_int64), ("seed", C.c_uint64), ("stochastic", C.c_int), ("step_ptr", C.c_void_p), ("lr_ptr", C.c_void_p),
+                ("grad_scale", C.c_void_p)]
 
 
 class CclError(RuntimeError):
@@ -85,6 +100,20 @@ def lib():
     L.mi_ccl_fusion_unpack.argtypes = [vp, vp, vp, vp]
     L.mi_ccl_fusion_reduce.argtypes = [vp, i, vp, vp, i, vp, i, i, i, vp]
     L.mi_ccl_fusion_reduce_static.argtypes = [vp, sz, i, sz, i, vp, vp, i, vp, i, i, i, vp]
+    L.mi_ccl_fusion_plan_elements.restype = sz
+    L.mi_ccl_fusion_plan_elements.argtypes = [vp]
+    L.mi_ccl_fusion_norm_workspace.restype = sz
+    L.mi_ccl_fusion_norm_workspace.argtypes = [vp]
+    L.mi_ccl_fusion_norm.argtypes = [vp, vp, vp, C.c_double, C.c_double, vp, vp, sz, vp]
+    L.mi_ccl_fusion_adamw.argtypes = [vp, i, vp, vp, vp, i, vp, vp, vp, vp, C.POINTER(AdamwOptions), vp]
+    L.mi_ccl_fusion_state_decode.argtypes = [vp, vp, vp, vp, i, vp, vp, vp]
+    L.mi_ccl_fusion_state_encode.argtypes = [vp, i, vp, vp, vp, vp, vp, vp]
+    L.mi_ccl_token_rows.argtypes = [sz, i, i, sz, sz, C.POINTER(sz)]
+    L.mi_ccl_token_sort_workspace.argtypes = [sz, i, i, C.POINTER(sz)]
+    L.mi_ccl_token_sort.argtypes = [i, vp, sz, i, i, sz, sz, vp, vp, vp, vp, sz, vp]
+    L.mi_ccl_token_dispatch.argtypes = [i, vp, sz, sz, i, sz, vp, vp, vp, i, vp, sz, sz, vp]
+    L.mi_ccl_token_combine.argtypes = [i, vp, sz, sz, vp, vp, sz, i, sz, vp, sz, vp]
+    L.mi_ccl_token_combine_backward.argtypes = [i, vp, sz, vp, sz, sz, vp, vp, vp, vp, i, sz, i, sz, vp, sz, vp, vp]
     L.mi_ccl_probe_bandwidth.argtypes = [i, vp, i, sz, vp]
     L.mi_ccl_last_kernel.restype = C.c_char_p
     L.mi_ccl_last_kernel.argtypes = []
@@ -122,6 +151,38 @@ def _stream(stream):
 
 def _ptr_array(xs):
     return (C.c_void_p * len(xs))(*[_ptr(x) for x in xs])
+
+
+_TORCH_DTYPE = {INT32: "int32", INT64: "int64", FLOAT16: "float16", FLOAT32: "float32", BFLOAT16: "bfloat16"}
+_CCL_DTYPE = {v: k for k, v in _TORCH_DTYPE.items()}
+
+
+def _dtype_name(t):
+    name = str(t.dtype).replace("torch.", "")
+    if name not in _CCL_DTYPE and name != "uint8":
+        raise ValueError(f"tensors of {name} are not taken")
+    return name
+
+
+def _ptr_or_none(x):
+    return None if x is None else _ptr(x)
+
+
+def _check_tensors(what, tensors, dtype=None, least=0):
+    """Raises unless every tensor is contiguous memory of the current GPU, of the dtype and with at least `least` elements."""
+    import torch
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is None:
+            raise ValueError(f"{what}: missing")
+        if not t.is_cuda or t.device.index != here:
+            raise ValueError(f"{what}: on {t.device}, the current device is cuda:{here}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: not contiguous")
+        if dtype is not None and str(t.dtype) != "torch." + dtype:
+            raise ValueError(f"{what}: {t.dtype}, {dtype} is wanted")
+        if t.numel() < least:
+            raise ValueError(f"{what}: {t.numel()} elements, {least} are needed")
 
 
 def datatype_size(dtype):
@@ -286,6 +347,80 @@ class FusionPlan:
                                           _ptr_array(out_tensors), lp_mode, bf16_impl, fp16_impl, _stream(stream)),
                "mi_ccl_fusion_reduce")
 
+    # ---- the optimizer step behind the reduce: gradients are the plan's tensors (a list) or its fusion buffer (one tensor) ----
+
+    @property
+    def elements(self):
+        """Elements of a state or fp32 copy of the weights in the plan's layout."""
+        return lib().mi_ccl_fusion_plan_elements(self._h)
+
+    def _gradients(self, grads):
+        if isinstance(grads, (list, tuple)):
+            if len(grads) != self.k or any(t.numel() < c for t, c in zip(grads, self.counts)):
+                raise ValueError("the gradients are not the plan's tensors")
+            _check_tensors("gradients", grads, _TORCH_DTYPE[self.dtype])
+            return _ptr_array(grads), None
+        _check_tensors("gradients", [grads], _TORCH_DTYPE[self.dtype], self.elements)
+        return None, _ptr(grads)
+
+    def norm(self, grads, result, multiplier=1.0, max_norm=0.0, workspace=None, stream=None):
+        """result[0] = the norm of all gradients times `multiplier`, result[1] = the factor of a clipped step's gradients (two
+        floats on the device).  workspace: norm_workspace bytes of device memory; allocated for the call when None."""
+        import torch
+        _check_tensors("result", [result], "float32", 2)
+        if workspace is None:
+            workspace = torch.empty(self.norm_workspace, dtype=torch.uint8, device=result.device)
+        _check_tensors("workspace", [workspace])
+        lst, buf = self._gradients(grads)
+        _check(lib().mi_ccl_fusion_norm(self._h, lst, buf, multiplier, max_norm, _ptr(result), _ptr(workspace),
+                                        workspace.numel() * workspace.element_size(), _stream(stream)), "mi_ccl_fusion_norm")
+
+    @property
+    def norm_workspace(self):
+        return lib().mi_ccl_fusion_norm_workspace(self._h)
+
+    def adamw(self, params, grads, exp_avg, exp_avg_sq, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, step=1, scales=None,
+              master=None, grad_scale=None, seed=None, step_ptr=None, lr_ptr=None, stream=None):
+        """One AdamW step over the plan's tensors, in place.  States: float32 (32 bits) or uint8 (8 bits, with `scales`) in the
+        plan's layout.  seed: not None rounds 8-bit states stochastically.  step_ptr (int64), lr_ptr and grad_scale (float32):
+        one-element device tensors read by the kernel."""
+        if len(params) != self.k or any(t.numel() < c for t, c in zip(params, self.counts)):
+            raise ValueError("the parameters are not the plan's tensors")
+        kind = _dtype_name(params[0])
+        _check_tensors("params", params, kind)
+        eight = _dtype_name(exp_avg) == "uint8"
+        _check_tensors("states", [exp_avg, exp_avg_sq], "uint8" if eight else "float32", self.elements)
+        if eight:
+            _check_tensors("scales", [scales], "uint8", 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK))
+        if master is not None:
+            _check_tensors("master", [master], "float32", self.elements)
+        for name, t, dt in (("grad_scale", grad_scale, "float32"), ("step_ptr", step_ptr, "int64"), ("lr_ptr", lr_ptr, "float32")):
+            if t is not None:
+                _check_tensors(name, [t], dt, 1)
+        lst, buf = self._gradients(grads)
+        o = AdamwOptions(lr, beta1, beta2, eps, weight_decay, int(step), 0 if seed is None else int(seed), int(seed is not None),
+                         _ptr_or_none(step_ptr), _ptr_or_none(lr_ptr), _ptr_or_none(grad_scale))
+        _check(lib().mi_ccl_fusion_adamw(self._h, _CCL_DTYPE[kind], _ptr_array(params), lst, buf, STATE_8BIT if eight else STATE_FP32,
+                                         _ptr(exp_avg), _ptr(exp_avg_sq), _ptr_or_none(scales), _ptr_or_none(master), C.byref(o),
+                                         _stream(stream)), "mi_ccl_fusion_adamw")
+
+    def _state_tensors(self, exp_avg, exp_avg_sq, scales, values_avg, values_sq):
+        _check_tensors("states", [exp_avg, exp_avg_sq], "uint8", self.elements)
+        _check_tensors("scales", [scales], "uint8", 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK))
+        _check_tensors("values", [values_avg, values_sq], _dtype_name(values_avg), self.elements)
+
+    def state_decode(self, exp_avg, exp_avg_sq, scales, values_avg, values_sq, stream=None):
+        """The values of 8-bit states, float32 or bfloat16."""
+        self._state_tensors(exp_avg, exp_avg_sq, scales, values_avg, values_sq)
+        _check(lib().mi_ccl_fusion_state_decode(self._h, _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(scales), _CCL_DTYPE[_dtype_name(values_avg)],
+                                                _ptr(values_avg), _ptr(values_sq), _stream(stream)), "mi_ccl_fusion_state_decode")
+
+    def state_encode(self, values_avg, values_sq, exp_avg, exp_avg_sq, scales, stream=None):
+        """Values (float32 or bfloat16) to 8-bit states, rounded to nearest."""
+        self._state_tensors(exp_avg, exp_avg_sq, scales, values_avg, values_sq)
+        _check(lib().mi_ccl_fusion_state_encode(self._h, _CCL_DTYPE[_dtype_name(values_avg)], _ptr(values_avg), _ptr(values_sq), _ptr(exp_avg),
+                                                _ptr(exp_avg_sq), _ptr(scales), _stream(stream)), "mi_ccl_fusion_state_encode")
+
     def close(self):
         if self._h:
             lib().mi_ccl_fusion_plan_destroy(self._h)
@@ -309,6 +444,120 @@ def fusion_reduce_static(counts, dtype, align, op, own_tensors, peers, out_tenso
     _check(lib().mi_ccl_fusion_reduce_static(cnt, k, dtype, align, op, _ptr_array(own_tensors), _ptr_array(peers),
                                              len(peers), _ptr_array(out_tensors), lp_mode, bf16_impl, fp16_impl,
                                              _stream(stream)), "mi_ccl_fusion_reduce_static")
+
+
+# ---- tokens sorted by expert, and back --------------------------------------------------------------------------------
+
+def _check_rows(what, t, hidden=None, dtype=None):
+    """(dtype, elements between rows) of a matrix of rows, whose rows are contiguous."""
+    import torch
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (hidden is not None and t.shape[1] != hidden):
+        raise ValueError(f"{what}: rows of {'contiguous' if hidden is None else hidden} elements are wanted, got {tuple(t.shape)}, strides {t.stride()}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    name = _dtype_name(t)
+    if dtype is not None and name != dtype:
+        raise ValueError(f"{what}: {name}, {dtype} is wanted")
+    # one row, or none, has no distance to the next
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.shape[0] > 1 and ld < t.shape[1]:
+        raise ValueError(f"{what}: rows overlap (strides {t.stride()})")
+    return name, ld
+
+
+def token_rows(n_tokens, top_k, n_experts, align=1, capacity=0):
+    """Most rows that the sorted buffer can take."""
+    r = C.c_size_t()
+    _check(lib().mi_ccl_token_rows(n_tokens, top_k, n_experts, align, capacity, C.byref(r)), "mi_ccl_token_rows")
+    return r.value
+
+
+def token_sort_workspace(n_tokens, top_k, n_experts):
+    r = C.c_size_t()
+    _check(lib().mi_ccl_token_sort_workspace(n_tokens, top_k, n_experts, C.byref(r)), "mi_ccl_token_sort_workspace")
+    return r.value
+
+
+def token_sort(expert_ids, n_experts, positions, counts, offsets, align=1, capacity=0, workspace=None, stream=None):
+    """Row of every entry of expert_ids [tokens, top_k] (int32 or int64) in the buffer sorted by expert, into positions (int32,
+    the same shape; -1: none); rows of each expert into counts, first rows and the end into offsets [n_experts + 1] (int32).
+    workspace: token_sort_workspace bytes; allocated for the call when None."""
+    import torch
+    if expert_ids.dim() != 2 or tuple(positions.shape) != tuple(expert_ids.shape):
+        raise ValueError("expert_ids and positions are [tokens, top_k]")
+    n, k = expert_ids.shape
+    _check_tensors("expert_ids", [expert_ids])
+    _check_tensors("positions", [positions], "int32")
+    _check_tensors("counts", [counts], "int32", n_experts)
+    _check_tensors("offsets", [offsets], "int32", n_experts + 1)
+    if workspace is None:
+        need = token_sort_workspace(n, k, n_experts)
+        workspace = torch.empty(need, dtype=torch.uint8, device=expert_ids.device) if need else None
+    size = 0
+    if workspace is not None:
+        _check_tensors("workspace", [workspace])
+        size = workspace.numel() * workspace.element_size()
+    _check(lib().mi_ccl_token_sort(_CCL_DTYPE.get(_dtype_name(expert_ids), -1), _ptr(expert_ids), n, k, n_experts, align, capacity,
+                                   _ptr(positions), _ptr(counts), _ptr(offsets), _ptr_or_none(workspace), size, _stream(stream)),
+           "mi_ccl_token_sort")
+
+
+def _check_segments(positions, counts, offsets, tokens):
+    _check_tensors("positions", [positions], "int32")
+    if positions.dim() != 2 or positions.shape[0] != tokens:
+        raise ValueError(f"positions: [{tokens}, top_k] is wanted, got {tuple(positions.shape)}")
+    if counts is not None:
+        _check_tensors("counts", [counts], "int32")
+        _check_tensors("offsets", [offsets], "int32", counts.numel() + 1)
+
+
+def token_dispatch(x, positions, counts, offsets, out, stream=None):
+    """out[positions[t, j]] = x[t]; padding rows become zero, rows behind the last expert's stay as they are."""
+    kind, ldx = _check_rows("x", x)
+    _, ldo = _check_rows("out", out, x.shape[1], kind)
+    _check_segments(positions, counts, offsets, x.shape[0])
+    _check(lib().mi_ccl_token_dispatch(_CCL_DTYPE.get(kind, -1), _ptr(x), ldx, x.shape[0], positions.shape[1], x.shape[1], _ptr(positions),
+                                       _ptr(counts), _ptr(offsets), counts.numel(), _ptr(out), ldo, out.shape[0], _stream(stream)),
+           "mi_ccl_token_dispatch")
+
+
+def token_combine(y, positions, weights, out, stream=None):
+    """out[t] = sum over j of weights[t, j] * y[positions[t, j]]; weights (float32, the shape of positions) may be None for ones."""
+    kind, ldy = _check_rows("y", y)
+    _, ldo = _check_rows("out", out, y.shape[1], kind)
+    _check_segments(positions, None, None, out.shape[0])
+    if weights is not None:
+        _check_tensors("weights", [weights], "float32", positions.numel())
+    _check(lib().mi_ccl_token_combine(_CCL_DTYPE.get(kind, -1), _ptr(y), ldy, y.shape[0], _ptr(positions), _ptr_or_none(weights),
+                                      out.shape[0], positions.shape[1], y.shape[1], _ptr(out), ldo, _stream(stream)), "mi_ccl_token_combine")
+
+
+def token_combine_backward(grad_out, y, positions, weights, counts, offsets, grad_y, grad_weights=None, stream=None):
+    """The gradient of token_combine: grad_y[positions[t, j]] = weights[t, j] * grad_out[t], with padding rows zero, and unless
+    None grad_weights[t, j] = <grad_out[t], y[positions[t, j]]>.  y may be None without grad_weights."""
+    kind, ldg = _check_rows("grad_out", grad_out)
+    hidden = grad_out.shape[1]
+    _, ldd = _check_rows("grad_y", grad_y, hidden, kind)
+    ldy = hidden
+    if y is not None:
+        _, ldy = _check_rows("y", y, hidden, kind)
+        if y.shape[0] != grad_y.shape[0]:
+            raise ValueError(f"y has {y.shape[0]} rows, grad_y {grad_y.shape[0]}")
+    elif grad_weights is not None:
+        raise ValueError("grad_weights needs y")
+    _check_segments(positions, counts, offsets, grad_out.shape[0])
+    for name, t in (("weights", weights), ("grad_weights", grad_weights)):
+        if t is not None:
+            _check_tensors(name, [t], "float32", positions.numel())
+    _check(lib().mi_ccl_token_combine_backward(_CCL_DTYPE.get(kind, -1), _ptr(grad_out), ldg, _ptr_or_none(y), ldy, grad_y.shape[0],
+                                               _ptr(positions), _ptr_or_none(weights), _ptr(counts), _ptr(offsets), counts.numel(),
+                                               grad_out.shape[0], positions.shape[1], hidden, _ptr(grad_y), ldd,
+                                               _ptr_or_none(grad_weights), _stream(stream)), "mi_ccl_token_combine_backward")
+
+
+def token_dispatch_backward(grad_rows, positions, grad_x, stream=None):
+    """The gradient of token_dispatch: grad_x[t] = sum over j of grad_rows[positions[t, j]]."""
+    token_combine(grad_rows, positions, None, grad_x, stream)
 
 
 PROBE_READ, PROBE_WRITE_ONE, PROBE_WRITE_FOUR = 0, 1, 2

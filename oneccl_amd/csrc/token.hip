@@ -1,0 +1,271 @@
+// Entry points of the token operators (sort, dispatch, combine and its gradient) in libmi_ccl_comp.so.
+#include <hip/hip_runtime.h>
+
+#include "../../include/mi_ccl_comp.h"
+#include "fusion_plan.hpp"
+#include "token_kernels.hpp"
+
+using namespace mi;
+
+namespace {
+
+constexpr uint64_t kMaxRows = 0x7fffffffull;       // positions are int32
+
+bool float_type(int dtype) {
+    return dtype == MI_CCL_FLOAT32 || dtype == MI_CCL_FLOAT16 || dtype == MI_CCL_BFLOAT16;
+}
+
+// n_tokens x top_k entries and an upper bound of the sorted buffer's rows; false where they do not fit
+bool token_sizes(size_t n_tokens, int top_k, int n_experts, size_t align, size_t capacity, uint64_t* entries, uint64_t* rows) {
+    if (top_k < 1 || n_experts < 1 || n_experts > kSortMaxExperts || align < 1 || align > kMaxRows || capacity > kMaxRows ||
+        n_tokens > kMaxRows / (uint64_t)top_k)
+        return false;
+    *entries = (uint64_t)n_tokens * (uint64_t)top_k;
+    uint64_t kept = *entries;
+    if (capacity && capacity * (uint64_t)n_experts < kept) kept = capacity * (uint64_t)n_experts;
+    // an expert with rows is padded by at most align - 1
+    const uint64_t padded = kept < (uint64_t)n_experts ? kept : (uint64_t)n_experts;
+    *rows = kept + padded * (align - 1);
+    return *rows <= kMaxRows;
+}
+
+bool row_pointer_ok(const void* p, int dtype) {
+    return p && (uintptr_t)p % fusion_dtype_size(dtype) == 0;
+}
+
+// positions, counts, offsets and fp32 weights, some of which may be NULL
+bool words_aligned(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr, const void* e = nullptr) {
+    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d | (uintptr_t)e) & 3u) == 0;
+}
+
+// How rows of `hidden` elements are shared out: U vectors per lane, as many waves per token as its row fills, and column
+// tiles of one row side by side in the grid when there are too few tokens to fill the chip.
+RowShape row_shape(size_t hidden, int dtype, size_t n_tokens, int top_k, int u) {
+    RowShape s;
+    const uint32_t vec = 16 / (uint32_t)fusion_dtype_size(dtype);
+    s.nvec = (uint32_t)(hidden / vec);
+    s.tail = (uint32_t)(hidden % vec);
+    s.log_waves = 0;
+    while (s.log_waves < 2 && (64u << s.log_waves) * u < s.nvec) s.log_waves++;
+    const uint32_t width = (64u << s.log_waves) * u;
+    s.cols = s.nvec ? (s.nvec + width - 1) / width : 1;
+    s.top_k = (uint32_t)top_k;
+    s.tokens = n_tokens;
+    return s;
+}
+
+constexpr uint64_t kTokenBlockLimit = 1u << 20;     // blocks along x: a block takes more tokens beyond
+
+uint32_t token_grid(const RowShape& s) {
+    const uint64_t per_block = (kBlock / 64) >> s.log_waves;
+    const uint64_t b = (s.tokens + per_block - 1) / per_block;
+    return (uint32_t)(b < kTokenBlockLimit ? b : kTokenBlockLimit);
+}
+
+// blocks along y: HIP allows 65535, a block takes more column tiles beyond
+uint32_t grid_columns(const RowShape& s) {
+    return s.cols < 65535u ? s.cols : 65535u;
+}
+
+int launched(const char* name) {
+    g_last_kernel = name;
+    return fusion_status_of(hipGetLastError());
+}
+
+template <class I>
+int sort_launch(const I* ids, uint32_t n, uint32_t experts, uint32_t align, uint32_t capacity, int32_t* positions, int32_t* counts,
+                int32_t* offsets, uint32_t* table, hipStream_t stream) {
+    const SortShape s = sort_shape(n);
+    if (s.runs > 1) {
+        hipLaunchKernelGGL((token_count_kernel<I>), dim3(s.runs), dim3(kSortBlock), 0, stream, ids, n, experts, s.run, table);
+        const int rc = launched("token_count_kernel");
+        if (rc != MI_CCL_SUCCESS) return rc;
+    }
+    if (experts <= 256)
+        hipLaunchKernelGGL((token_place_kernel<I, 256>), dim3(s.runs), dim3(kSortBlock), 0, stream, ids, n, experts, s.run, s.runs,
+                           (const uint32_t*)table, align, capacity, positions, counts, offsets);
+    else
+        hipLaunchKernelGGL((token_place_kernel<I, kSortMaxExperts>), dim3(s.runs), dim3(kSortBlock), 0, stream, ids, n, experts, s.run, s.runs,
+                           (const uint32_t*)table, align, capacity, positions, counts, offsets);
+    return launched("token_place_kernel");
+}
+
+constexpr int kDispatchU = 2;
+constexpr int kCombineU = 1;
+
+template <class E>
+void dispatch_launch(const RowShape& s, dim3 grid, uint32_t token_blocks, hipStream_t stream, const void* x, size_t ld_x, const int32_t* positions,
+                     const int32_t* counts, const int32_t* offsets, void* out, size_t ld_out, size_t rows) {
+    hipLaunchKernelGGL((token_dispatch_kernel<E, kDispatchU>), grid, dim3(kBlock), 0, stream, (const unsigned char*)x, (uint64_t)ld_x, s,
+                       token_blocks, positions, counts, offsets, (unsigned char*)out, (uint64_t)ld_out, (uint64_t)rows);
+}
+
+template <class V, int K>
+void combine_launch(const RowShape& s, hipStream_t stream, const void* y, size_t ld_y, size_t rows, const int32_t* positions,
+                    const float* weights, void* out, size_t ld_out) {
+    hipLaunchKernelGGL((token_combine_kernel<V, kCombineU, K>), dim3(token_grid(s), grid_columns(s)), dim3(kBlock), 0, stream, (const unsigned char*)y,
+                       (uint64_t)ld_y, (uint64_t)rows, s, positions, weights, (unsigned char*)out, (uint64_t)ld_out);
+}
+template <class V>
+void combine_by_k(const RowShape& s, hipStream_t stream, const void* y, size_t ld_y, size_t rows, const int32_t* positions,
+                  const float* weights, void* out, size_t ld_out) {
+    if (s.top_k == 1) combine_launch<V, 1>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    else if (s.top_k == 2) combine_launch<V, 2>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    else if (s.top_k <= 4) combine_launch<V, 4>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    else combine_launch<V, 8>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+}
+
+struct BackwardArgs {
+    RowShape s;
+    uint32_t block, token_blocks, grid;
+    hipStream_t stream;
+    const void *grad, *y;
+    size_t ld_grad, ld_y, ld_grad_y, rows;
+    const int32_t *positions, *counts, *offsets;
+    const float* weights;
+    void* grad_y;
+    float* grad_weights;
+};
+template <class V, int K, bool DOT>
+void backward_launch(const BackwardArgs& a) {
+    hipLaunchKernelGGL((token_combine_backward_kernel<V, K, DOT>), dim3(a.grid), dim3(a.block), 0, a.stream, (const unsigned char*)a.grad,
+                       (uint64_t)a.ld_grad, (const unsigned char*)a.y, (uint64_t)a.ld_y, (uint64_t)a.rows, a.s, a.token_blocks, a.positions,
+                       a.weights, a.counts, a.offsets, (unsigned char*)a.grad_y, (uint64_t)a.ld_grad_y, a.grad_weights);
+}
+template <class V, bool DOT>
+void backward_by_k(const BackwardArgs& a) {
+    if (a.s.top_k == 1) backward_launch<V, 1, DOT>(a);
+    else if (a.s.top_k == 2) backward_launch<V, 2, DOT>(a);
+    else if (a.s.top_k <= 4) backward_launch<V, 4, DOT>(a);
+    else backward_launch<V, 8, DOT>(a);
+}
+template <class V>
+void backward_by_dot(const BackwardArgs& a) {
+    if (a.grad_weights) backward_by_k<V, true>(a);
+    else backward_by_k<V, false>(a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mi_ccl_token_rows(size_t n_tokens, int top_k, int n_experts, size_t align, size_t capacity, size_t* rows) {
+    uint64_t entries = 0, r = 0;
+    if (!rows || !token_sizes(n_tokens, top_k, n_experts, align, capacity, &entries, &r))
+        return MI_CCL_INVALID_ARGUMENTS;
+    *rows = (size_t)r;
+    return MI_CCL_SUCCESS;
+}
+
+int mi_ccl_token_sort_workspace(size_t n_tokens, int top_k, int n_experts, size_t* bytes) {
+    uint64_t entries = 0, r = 0;
+    if (!bytes || !token_sizes(n_tokens, top_k, n_experts, 1, 0, &entries, &r))
+        return MI_CCL_INVALID_ARGUMENTS;
+    const SortShape s = sort_shape((uint32_t)entries);
+    *bytes = s.runs > 1 ? (size_t)s.runs * (size_t)n_experts * sizeof(uint32_t) : 0;
+    return MI_CCL_SUCCESS;
+}
+
+int mi_ccl_token_sort(int index_dtype, const void* expert_ids, size_t n_tokens, int top_k, int n_experts, size_t align, size_t capacity,
+                      int32_t* positions, int32_t* counts, int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream) {
+    uint64_t entries = 0, rows = 0;
+    size_t need = 0;
+    if ((index_dtype != MI_CCL_INT32 && index_dtype != MI_CCL_INT64) || !counts || !offsets ||
+        !token_sizes(n_tokens, top_k, n_experts, align, capacity, &entries, &rows))
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (entries && (!expert_ids || (uintptr_t)expert_ids % fusion_dtype_size(index_dtype) || !positions))
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (!words_aligned(positions, counts, offsets, workspace))
+        return MI_CCL_INVALID_ARGUMENTS;
+    mi_ccl_token_sort_workspace(n_tokens, top_k, n_experts, &need);
+    if (need && (!workspace || workspace_bytes < need))
+        return MI_CCL_INVALID_ARGUMENTS;
+    const uint32_t cap = capacity ? (uint32_t)capacity : 0xffffffffu;
+    if (index_dtype == MI_CCL_INT32)
+        return sort_launch<int32_t>((const int32_t*)expert_ids, (uint32_t)entries, (uint32_t)n_experts, (uint32_t)align, cap, positions, counts,
+                                    offsets, (uint32_t*)workspace, (hipStream_t)stream);
+    return sort_launch<int64_t>((const int64_t*)expert_ids, (uint32_t)entries, (uint32_t)n_experts, (uint32_t)align, cap, positions, counts,
+                                offsets, (uint32_t*)workspace, (hipStream_t)stream);
+}
+
+int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens, int top_k, size_t hidden, const int32_t* positions,
+                          const int32_t* counts, const int32_t* offsets, int n_experts, void* out, size_t ld_out, size_t out_rows,
+                          void* stream) {
+    if (!float_type(dtype) || top_k < 1 || n_experts < 1 || n_experts > kSortMaxExperts)
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (n_tokens == 0 || hidden == 0 || out_rows == 0)
+        return MI_CCL_SUCCESS;
+    if (!row_pointer_ok(x, dtype) || !row_pointer_ok(out, dtype) || !positions || !counts || !offsets || ld_x < hidden || ld_out < hidden ||
+        hidden > kMaxRows || n_tokens > kMaxRows / (uint64_t)top_k || out_rows > kMaxRows || !words_aligned(positions, counts, offsets))
+        return MI_CCL_INVALID_ARGUMENTS;
+    const RowShape s = row_shape(hidden, dtype, n_tokens, top_k, kDispatchU);
+    const uint32_t token_blocks = token_grid(s);
+    const dim3 grid(token_blocks + (uint32_t)n_experts, grid_columns(s));
+    if (fusion_dtype_size(dtype) == 4)
+        dispatch_launch<uint32_t>(s, grid, token_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
+    else
+        dispatch_launch<uint16_t>(s, grid, token_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
+    return launched("token_dispatch_kernel");
+}
+
+int mi_ccl_token_combine(int dtype, const void* y, size_t ld_y, size_t y_rows, const int32_t* positions, const float* weights,
+                         size_t n_tokens, int top_k, size_t hidden, void* out, size_t ld_out, void* stream) {
+    if (!float_type(dtype) || top_k < 1)
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (n_tokens == 0 || hidden == 0)
+        return MI_CCL_SUCCESS;
+    if ((y_rows && !row_pointer_ok(y, dtype)) || !row_pointer_ok(out, dtype) || !positions || ld_y < hidden || ld_out < hidden ||
+        hidden > kMaxRows || n_tokens > kMaxRows / (uint64_t)top_k || y_rows > kMaxRows || !words_aligned(positions, weights))
+        return MI_CCL_INVALID_ARGUMENTS;
+    const RowShape s = row_shape(hidden, dtype, n_tokens, top_k, kCombineU);
+    if (dtype == MI_CCL_FLOAT32) combine_by_k<F32Vec>(s, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
+    else if (dtype == MI_CCL_BFLOAT16) combine_by_k<Bf16Vec>(s, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
+    else combine_by_k<Fp16Vec>(s, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
+    return launched("token_combine_kernel");
+}
+
+int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_grad, const void* y, size_t ld_y, size_t y_rows,
+                                  const int32_t* positions, const float* weights, const int32_t* counts, const int32_t* offsets,
+                                  int n_experts, size_t n_tokens, int top_k, size_t hidden, void* grad_y, size_t ld_grad_y,
+                                  float* grad_weights, void* stream) {
+    if (!float_type(dtype) || top_k < 1 || n_experts < 1 || n_experts > kSortMaxExperts)
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (n_tokens == 0)
+        return MI_CCL_SUCCESS;
+    if (!positions || !counts || !offsets || hidden > kMaxRows || n_tokens > kMaxRows / (uint64_t)top_k || y_rows > kMaxRows ||
+        !words_aligned(positions, weights, counts, offsets, grad_weights))
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (hidden && (!row_pointer_ok(grad_out, dtype) || ld_grad < hidden))
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (hidden && y_rows && (!row_pointer_ok(grad_y, dtype) || ld_grad_y < hidden || (grad_weights && (!row_pointer_ok(y, dtype) || ld_y < hidden))))
+        return MI_CCL_INVALID_ARGUMENTS;
+    if (!grad_weights && (hidden == 0 || y_rows == 0))
+        return MI_CCL_SUCCESS;
+    BackwardArgs a;
+    a.s = row_shape(hidden, dtype, n_tokens, top_k, 1);
+    // a block per token: as many lanes as the row has vectors, at most 256; up to 1024 when there are too few tokens for the chip
+    const uint32_t most = n_tokens >= 256 ? 256 : 1024;
+    a.block = 64;
+    while (a.block < a.s.nvec && a.block < most) a.block <<= 1;
+    a.token_blocks = (uint32_t)(n_tokens < kTokenBlockLimit ? n_tokens : kTokenBlockLimit);
+    a.grid = a.token_blocks + (uint32_t)n_experts;
+    a.stream = (hipStream_t)stream;
+    a.grad = grad_out;
+    a.ld_grad = ld_grad;
+    a.y = y;
+    a.ld_y = ld_y;
+    a.rows = y_rows;
+    a.positions = positions;
+    a.weights = weights;
+    a.counts = counts;
+    a.offsets = offsets;
+    a.grad_y = grad_y;
+    a.ld_grad_y = ld_grad_y;
+    a.grad_weights = grad_weights;
+    if (dtype == MI_CCL_FLOAT32) backward_by_dot<F32Vec>(a);
+    else if (dtype == MI_CCL_BFLOAT16) backward_by_dot<Bf16Vec>(a);
+    else backward_by_dot<Fp16Vec>(a);
+    return launched("token_combine_backward_kernel");
+}
+
+} /* extern "C" */
