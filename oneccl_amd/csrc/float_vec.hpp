@@ -6,6 +6,8 @@
 
 namespace mi {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 struct F32Vec {
     typedef uint32_t elem_t;
     static constexpr int VEC = 4;
@@ -18,6 +20,8 @@ struct F32Vec {
     static __device__ __forceinline__ u32x4 narrow(const float* f) {
         return u32x4{ as_u32(f[0]), as_u32(f[1]), as_u32(f[2]), as_u32(f[3]) };
     }
+    static __device__ __forceinline__ void widen_half(u32x2, float*) {}         // four elements are a whole vector
+    static __device__ __forceinline__ u32x2 narrow_half(const float*) { return u32x2{ 0, 0 }; }
 };
 
 struct Bf16Vec {
@@ -31,6 +35,18 @@ struct Bf16Vec {
             f[2 * i] = as_f32(x[i] << 16);
             f[2 * i + 1] = as_f32(x[i] & 0xffff0000u);
         }
+    }
+    static __device__ __forceinline__ void widen_half(u32x2 x, float* f) {      // four elements
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            f[2 * i] = as_f32(x[i] << 16);
+            f[2 * i + 1] = as_f32(x[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x2 narrow_half(const float* f) {
+        const f32x2 a = { f[0], f[1] }, b = { f[2], f[3] };
+        return u32x2{ __builtin_bit_cast(uint32_t, __builtin_convertvector(a, bf16x2)),
+                      __builtin_bit_cast(uint32_t, __builtin_convertvector(b, bf16x2)) };
     }
     static __device__ __forceinline__ u32x4 narrow(const float* f) {
         u32x4 r;
@@ -57,6 +73,19 @@ struct Fp16Vec {
             f[2 * i] = (float)h[0];
             f[2 * i + 1] = (float)h[1];
         }
+    }
+    static __device__ __forceinline__ void widen_half(u32x2 x, float* f) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t d = x[i];
+            const half2 h = __builtin_bit_cast(half2, d);
+            f[2 * i] = (float)h[0];
+            f[2 * i + 1] = (float)h[1];
+        }
+    }
+    static __device__ __forceinline__ u32x2 narrow_half(const float* f) {
+        const half2 a = { (_Float16)f[0], (_Float16)f[1] }, b = { (_Float16)f[2], (_Float16)f[3] };
+        return u32x2{ __builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b) };
     }
     static __device__ __forceinline__ u32x4 narrow(const float* f) {
         u32x4 r;

@@ -71,7 +71,7 @@ struct AdamwLaunch {
 };
 template <class P, class G, bool MASTER, int STATE>
 hipError_t adamw_launch(const AdamwLaunch& a) {
-    hipLaunchKernelGGL((fusion_adamw_kernel<P, G, MASTER, STATE>), dim3(a.blocks), dim3(kBlock), 0, a.stream, *a.params, *a.grads, a.buffer, a.tb,
+    hipLaunchKernelGGL((fusion_adamw_kernel<P, G, MASTER, STATE>), dim3(a.blocks), dim3(AdamwShape<STATE>::block), 0, a.stream, *a.params, *a.grads, a.buffer, a.tb,
                        a.st, a.sc);
     return hipGetLastError();
 }
@@ -228,7 +228,7 @@ int mi_ccl_fusion_adamw(mi_ccl_fusion_plan* plan, int param_dtype, void* const* 
     adamw_derive(sc);
 
     const int state = !eight ? STATE_FP32 : o->stochastic ? STATE_RANDOM : STATE_NEAREST;
-    const uint32_t subs = kFusionChunk / (uint32_t)plan->esz / kOptTile;
+    const uint32_t subs = kFusionChunk / (uint32_t)plan->esz / kAdamwTile;
     const uint64_t most = items_per_launch(subs);
     for (size_t t0 = 0; t0 < plan->k; t0 += kFusionGroup) {
         const size_t t1 = (t0 + kFusionGroup < plan->k) ? t0 + kFusionGroup : plan->k;
@@ -254,7 +254,7 @@ int mi_ccl_fusion_state_decode(mi_ccl_fusion_plan* plan, const void* exp_avg, co
     if (rc != MI_CCL_SUCCESS)
         return rc;
     AdamwTables tb = plan_tables(plan);
-    const uint32_t elems = kFusionChunk / (uint32_t)plan->esz, subs = elems / kOptTile;
+    const uint32_t elems = kFusionChunk / (uint32_t)plan->esz, subs = elems / (kBlock * 4 * kDecodeGroups);
     const uint64_t most = items_per_launch(subs), all = plan->item_begin[plan->k];
     for (uint64_t i0 = 0; i0 < all; i0 += most) {
         tb.items = plan->d_items + i0;
@@ -279,7 +279,7 @@ int mi_ccl_fusion_state_encode(mi_ccl_fusion_plan* plan, int value_dtype, const 
     if (rc != MI_CCL_SUCCESS)
         return rc;
     AdamwTables tb = plan_tables(plan);
-    const uint32_t elems = kFusionChunk / (uint32_t)plan->esz, subs = elems / kOptTile;
+    const uint32_t elems = kFusionChunk / (uint32_t)plan->esz, subs = elems / (kBlock * 4 * kEncodeGroups);
     const uint64_t most = items_per_launch(subs), all = plan->item_begin[plan->k];
     for (uint64_t i0 = 0; i0 < all; i0 += most) {
         tb.items = plan->d_items + i0;

@@ -22,9 +22,8 @@
 namespace mi {
 
 constexpr uint32_t kStateBlock = MI_CCL_STATE_BLOCK;    // elements of one 8-bit block
-constexpr uint32_t kLaneElems = 8;                      // elements of one lane
-constexpr uint32_t kOptTile = kBlock * kLaneElems;      // elements of one block of threads
-static_assert(kOptTile % kStateBlock == 0 && kStateBlock == 32 * kLaneElems, "half a wave holds one 8-bit block");
+constexpr uint32_t kAdamwTile = 512;                    // elements of one block of threads of the AdamW step
+static_assert(kStateBlock == 64 * 4, "four elements of each lane of a wave are one 8-bit block");
 
 // ---- norm ---------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kNormBlocks = 2048;      // partial sums of one launch
@@ -109,10 +108,10 @@ fusion_norm_finish_kernel(const double* partial, uint32_t n, double multiplier, 
 
 // ---- 8-bit states -------------------------------------------------------------------------------------------------------
 
-// The largest of a value over the 32 lanes that hold one block.
+// The largest of a value over the wave, which holds one block.
 __device__ __forceinline__ float block_max(float x) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
+    for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
     return x;
 }
 __device__ __forceinline__ float finite_magnitude(float x) {
@@ -170,61 +169,62 @@ __device__ __forceinline__ uint32_t element_random(uint64_t index, uint32_t key)
     return mix32((uint32_t)index ^ key ^ ((uint32_t)(index >> 32) * 0x85EBCA77u));
 }
 
-// ---- a lane's eight elements ----------------------------------------------------------------------------------------------
+// ---- a lane's elements ----------------------------------------------------------------------------------------------------
 
-template <class V>
-__device__ __forceinline__ void load8(const void* p, uint32_t n, float* f) {
-    typedef typename V::elem_t E;
-    constexpr int VEC = V::VEC;
-    if (n == kLaneElems) {
-#pragma unroll
-        for (int q = 0; q < (int)kLaneElems / VEC; q++) V::widen(ld_loose((const u32x4_u*)p + q), f + q * VEC);
-    }
-    else {
-#pragma unroll
-        for (uint32_t i = 0; i < kLaneElems; i++) f[i] = i < n ? V::widen1(ld_elem<E>(p, i)) : 0.0f;
-    }
-}
-template <class V>
-__device__ __forceinline__ void store8(void* p, uint32_t n, const float* f) {
-    typedef typename V::elem_t E;
-    constexpr int VEC = V::VEC;
-    if (n == kLaneElems) {
-#pragma unroll
-        for (int q = 0; q < (int)kLaneElems / VEC; q++) st_loose((u32x4_u*)p + q, V::narrow(f + q * VEC));
-    }
-    else {
-#pragma unroll
-        for (uint32_t i = 0; i < kLaneElems; i++)
-            if (i < n) st_elem<E>(p, i, V::narrow1(f[i]));
-    }
-}
-// eight codes; a block starts on a multiple of 256 codes, so whole groups are aligned to the base's alignment
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// Four elements of consecutive memory, as many bytes as their type needs (16, 8 or 4): with lane after lane behind each other
+// every access of a wave covers one unbroken run, whatever the widths of the arrays that meet in one element are.
 typedef u32x2 u32x2_u __attribute__((aligned(1)));
-__device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t n, uint32_t* c) {
-    if (n == kLaneElems) {
-        const u32x2 x = __builtin_nontemporal_load((const u32x2_u*)p);
-#pragma unroll
-        for (int i = 0; i < 8; i++) c[i] = (x[i / 4] >> (8 * (i & 3))) & 0xffu;
+typedef uint32_t u32_u __attribute__((aligned(1)));
+
+// WHOLE: all four, else elements [from, to) of them (none when from >= to).
+struct Span {
+    int from, to;
+    __device__ __forceinline__ bool has(int i) const { return i >= from && i < to; }
+    __device__ __forceinline__ bool whole() const { return from <= 0 && to >= 4; }
+};
+template <class V, bool WHOLE>
+__device__ __forceinline__ void load4(const void* p, Span n, float* f) {
+    typedef typename V::elem_t E;
+    if (WHOLE || n.whole()) {
+        if (sizeof(E) == 4) V::widen(ld_loose((const u32x4_u*)p), f);
+        else V::widen_half(__builtin_nontemporal_load((const u32x2_u*)p), f);
     }
     else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) c[i] = i < n ? p[i] : 0;
+        for (int i = 0; i < 4; i++) f[i] = n.has(i) ? V::widen1(ld_elem<E>(p, i)) : 0.0f;
     }
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, uint32_t n, const uint32_t* c) {
-    if (n == kLaneElems) {
-        u32x2 x = { 0, 0 };
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i / 4] |= c[i] << (8 * (i & 3));
-        __builtin_nontemporal_store(x, (u32x2_u*)p);
+template <class V, bool WHOLE>
+__device__ __forceinline__ void store4(void* p, Span n, const float* f) {
+    typedef typename V::elem_t E;
+    if (WHOLE || n.whole()) {
+        if (sizeof(E) == 4) st_loose((u32x4_u*)p, V::narrow(f));
+        else __builtin_nontemporal_store(V::narrow_half(f), (u32x2_u*)p);
     }
     else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++)
-            if (i < n) p[i] = (uint8_t)c[i];
+        for (int i = 0; i < 4; i++)
+            if (n.has(i)) st_elem<E>(p, i, V::narrow1(f[i]));
     }
+}
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, Span n) {
+    if (WHOLE || n.whole()) return __builtin_nontemporal_load((const u32_u*)p);
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (n.has(i)) c |= (uint32_t)p[i] << (8 * i);
+    return c;
+}
+template <bool WHOLE>
+__device__ __forceinline__ void store_codes(uint8_t* p, Span n, uint32_t c) {
+    if (WHOLE || n.whole()) {
+        __builtin_nontemporal_store(c, (u32_u*)p);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (n.has(i)) p[i] = (uint8_t)(c >> (8 * i));
 }
 
 // ---- AdamW --------------------------------------------------------------------------------------------------------------
@@ -274,14 +274,138 @@ struct AdamwState {
     float* master;
 };
 
+// sqrt to one ulp: v_sqrt_f32, whose argument may not be denormal, hence the detour for the smallest; `scale` is a factor of
+// the result.
+__device__ __forceinline__ float scaled_sqrt(float v, float scale) {
+    const bool tiny = v < 0x1p-96f;
+    return __builtin_amdgcn_sqrtf(v * (tiny ? 0x1p64f : 1.0f)) * (tiny ? scale * 0x1p-32f : scale);
+}
+// One element's step: m, v and x (the weight) in, out.
+__device__ __forceinline__ void adamw_element(const AdamwScalars& a, float g, float& m, float& v, float& x) {
+    m = m * a.beta1 + g * a.rest1;
+    v = v * a.beta2 + (g * g) * a.rest2;
+    const float root = scaled_sqrt(v, a.root_scale) + a.eps;
+    x = x * a.decay - (m * __builtin_amdgcn_rcpf(root)) * a.step_size;
+}
+
+// A tensor's arrays, each at the tensor's element 0.
+struct AdamwTensor {
+    unsigned char* p;
+    const unsigned char* g;
+    float* master;
+    void* avg;
+    void* sq;
+    uint8_t* scales;
+    uint64_t at;                // element 0 in the plan's layout
+    int64_t count;
+};
+
 enum { STATE_FP32 = 0, STATE_NEAREST = 1, STATE_RANDOM = 2 };
 
-// A block of threads takes 2048 elements of one item, a lane eight of them in a row.
+// Groups of four elements of a lane, and lanes of a block.  Small blocks that read once and write once are what the memory
+// system takes best (200 M parameters with 32-bit states, tight layout: 959 us, against 998 with 1,024 elements and 1,018 with
+// 2,048 per block); 8-bit states gain from a second group per lane (130 M parameters: 349 against 357 us), which shares the
+// tile's bookkeeping.
+template <int STATE>
+struct AdamwShape {
+    static constexpr uint32_t groups = STATE == STATE_FP32 ? 1 : 2;
+    static constexpr uint32_t block = kAdamwTile / (4 * groups);
+};
+
+// Elements [e0, e0 + kAdamwTile) of a tensor, those that it has (WHOLE: all of them).
+template <class P, class G, bool MASTER, int STATE, bool WHOLE>
+__device__ __forceinline__ void adamw_tile(const AdamwTensor& t, int64_t e0, const AdamwScalars& a, float scale) {
+    constexpr int64_t GS = sizeof(typename G::elem_t), PS = sizeof(typename P::elem_t);
+    constexpr uint32_t kGroups = AdamwShape<STATE>::groups;
+    Span n[kGroups];                                            // what the lane has of its groups of four
+    float g[kGroups][4], m[kGroups][4], v[kGroups][4], x[kGroups][4];
+    uint32_t cm[kGroups], cv[kGroups], sm[kGroups], sv[kGroups];
+    unsigned char* const p0 = t.p + e0 * PS;
+    const unsigned char* const g0 = t.g + e0 * GS;
+    float* const master = t.master + e0;
+    float* const avg = (float*)t.avg + e0;
+    float* const sq = (float*)t.sq + e0;
+    uint8_t* const avg8 = (uint8_t*)t.avg + e0;
+    uint8_t* const sq8 = (uint8_t*)t.sq + e0;
+    uint8_t* const scales = t.scales + 2 * (e0 / kStateBlock);
+#pragma unroll
+    for (uint32_t q = 0; q < kGroups; q++) {
+        const uint32_t e = (threadIdx.x >> 6) * (256 * kGroups) + q * 256 + (threadIdx.x & 63u) * 4;
+        n[q] = Span{ 0, 4 };
+        if (!WHOLE) {
+            const int64_t lo = -(e0 + e), hi = t.count - (e0 + e);
+            n[q].from = lo > 4 ? 4 : lo < 0 ? 0 : (int)lo;
+            n[q].to = hi > 4 ? 4 : hi < 0 ? 0 : (int)hi;
+            if (n[q].from >= n[q].to) n[q] = Span{ 4, 0 };
+        }
+        load4<G, WHOLE>(g0 + e * GS, n[q], g[q]);
+        if (MASTER) load4<F32Vec, WHOLE>(master + e, n[q], x[q]);
+        else load4<P, WHOLE>(p0 + e * PS, n[q], x[q]);
+        if (STATE == STATE_FP32) {
+            load4<F32Vec, WHOLE>(avg + e, n[q], m[q]);
+            load4<F32Vec, WHOLE>(sq + e, n[q], v[q]);
+        }
+        else {
+            cm[q] = load_codes<WHOLE>(avg8 + e, n[q]);
+            cv[q] = load_codes<WHOLE>(sq8 + e, n[q]);
+            sm[q] = sv[q] = 0;
+            if (WHOLE || n[q].to) {
+                sm[q] = scales[2 * (e / kStateBlock)];
+                sv[q] = scales[2 * (e / kStateBlock) + 1];
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < kGroups; q++) {
+        const uint32_t e = (threadIdx.x >> 6) * (256 * kGroups) + q * 256 + (threadIdx.x & 63u) * 4;
+        float lm = 0.0f, lv = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (STATE != STATE_FP32) {
+                m[q][i] = value_avg((cm[q] >> (8 * i)) & 0xffu, sm[q]);
+                v[q][i] = value_sq((cv[q] >> (8 * i)) & 0xffu, sv[q]);
+            }
+            adamw_element(a, g[q][i] * scale, m[q][i], v[q][i], x[q][i]);
+            if (STATE != STATE_FP32 && (WHOLE || n[q].has(i))) {
+                lm = fmaxf(lm, finite_magnitude(m[q][i]));
+                lv = fmaxf(lv, finite_magnitude(v[q][i]));
+            }
+        }
+        if (MASTER) store4<F32Vec, WHOLE>(master + e, n[q], x[q]);
+        store4<P, WHOLE>(p0 + e * PS, n[q], x[q]);
+        if (STATE == STATE_FP32) {
+            store4<F32Vec, WHOLE>(avg + e, n[q], m[q]);
+            store4<F32Vec, WHOLE>(sq + e, n[q], v[q]);
+        }
+        else {
+            const uint32_t tm = scale_avg(block_max(lm)), tv = scale_sq(block_max(lv));
+            uint32_t om = 0, ov = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t r = STATE == STATE_RANDOM ? element_random(t.at + e0 + e + i, a.key) : 0;
+                om |= code_avg<STATE == STATE_RANDOM>(m[q][i], tm, r & 0xffffu) << (8 * i);
+                ov |= code_sq<STATE == STATE_RANDOM>(v[q][i], tv, r >> 16) << (8 * i);
+            }
+            store_codes<WHOLE>(avg8 + e, n[q], om);
+            store_codes<WHOLE>(sq8 + e, n[q], ov);
+            if ((WHOLE || n[q].to) && (threadIdx.x & 63u) == 0) {
+                scales[2 * (e / kStateBlock)] = (uint8_t)tm;
+                scales[2 * (e / kStateBlock) + 1] = (uint8_t)tv;
+            }
+        }
+    }
+}
+
+// A block of threads takes kAdamwTile elements of a tensor, a wave a run of 256 times the groups of a lane, which are four in a
+// row: one 8-bit block is one group of all 64 lanes, and every access of a wave is one unbroken run.
+// With 32-bit states in a tight layout a tensor may start anywhere in its arrays.  The tiles are cut where the states cross a
+// 256-byte boundary, `back` elements before the multiples of kAdamwTile, so that no two blocks write to one line; tile 0 has
+// `back` elements less, and the tensor's last block takes a second, short tile when that leaves elements over.
 template <class P, class G, bool MASTER, int STATE>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(AdamwShape<STATE>::block)
 fusion_adamw_kernel(FusionPtrs params, FusionPtrs grads, const unsigned char* buffer, AdamwTables tb, AdamwState st, AdamwScalars a) {
-    constexpr uint32_t GS = sizeof(typename G::elem_t), PS = sizeof(typename P::elem_t);
-    constexpr uint32_t kItemElems = kFusionChunk / GS, kSubs = kItemElems / kOptTile;
+    constexpr uint32_t GS = sizeof(typename G::elem_t);
+    constexpr uint32_t kItemElems = kFusionChunk / GS, kSubs = kItemElems / kAdamwTile;
     float scale = 1.0f;
     if (a.grad_scale) {
         scale = *a.grad_scale;
@@ -293,105 +417,80 @@ fusion_adamw_kernel(FusionPtrs params, FusionPtrs grads, const unsigned char* bu
         adamw_derive(a);
     }
     const FusionItem w = tb.items[blockIdx.x / kSubs];
-    const uint64_t e0 = (uint64_t)w.c * kItemElems + (blockIdx.x % kSubs) * kOptTile;
-    const uint64_t count = tb.bytes[w.t] / GS;
-    if (e0 >= count) return;
-    const uint64_t e = e0 + threadIdx.x * kLaneElems;
-    const uint32_t n = e >= count ? 0u : count - e < kLaneElems ? (uint32_t)(count - e) : kLaneElems;
-    const uint64_t at = tb.off[w.t] / GS + e;                   // the lane's first element in the plan's layout
-    unsigned char* p = (unsigned char*)(uintptr_t)params.get(w.t - tb.t0) + e * PS;
-    const unsigned char* gp = (buffer ? buffer + tb.off[w.t] : (const unsigned char*)(uintptr_t)grads.get(w.t - tb.t0)) + e * GS;
-
-    float g[8], m[8], v[8], x[8];
-    load8<G>(gp, n, g);
-    if (MASTER) load8<F32Vec>(st.master + at, n, x);
-    else load8<P>(p, n, x);
-    if (STATE == STATE_FP32) {
-        load8<F32Vec>((const float*)st.avg + at, n, m);
-        load8<F32Vec>((const float*)st.sq + at, n, v);
-    }
-    else {
-        uint32_t cm[8], cv[8], sm = 0, sv = 0;
-        load_codes((const uint8_t*)st.avg + at, n, cm);
-        load_codes((const uint8_t*)st.sq + at, n, cv);
-        if (n) {
-            const uint8_t* s = st.scales + 2 * (at / kStateBlock);
-            sm = s[0];
-            sv = s[1];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            m[i] = value_avg(cm[i], sm);
-            v[i] = value_sq(cv[i], sv);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float gs = g[i] * scale;
-        m[i] = m[i] * a.beta1 + gs * a.rest1;
-        v[i] = v[i] * a.beta2 + (gs * gs) * a.rest2;
-        const float root = sqrtf(v[i]) * a.root_scale + a.eps;
-        x[i] = x[i] * a.decay - (m[i] / root) * a.step_size;
-    }
-    if (MASTER) store8<F32Vec>(st.master + at, n, x);
-    store8<P>(p, n, x);
-    if (STATE == STATE_FP32) {
-        store8<F32Vec>((float*)st.avg + at, n, m);
-        store8<F32Vec>((float*)st.sq + at, n, v);
-    }
-    else {
-        float lm = 0.0f, lv = 0.0f;
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            if (i < n) {
-                lm = fmaxf(lm, finite_magnitude(m[i]));
-                lv = fmaxf(lv, finite_magnitude(v[i]));
-            }
-        }
-        const uint32_t sm = scale_avg(block_max(lm)), sv = scale_sq(block_max(lv));
-        uint32_t cm[8], cv[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t r = STATE == STATE_RANDOM ? element_random(at + i, a.key) : 0;
-            cm[i] = code_avg<STATE == STATE_RANDOM>(m[i], sm, r & 0xffffu);
-            cv[i] = code_sq<STATE == STATE_RANDOM>(v[i], sv, r >> 16);
-        }
-        store_codes((uint8_t*)st.avg + at, n, cm);
-        store_codes((uint8_t*)st.sq + at, n, cv);
-        if (n && (threadIdx.x & 31u) == 0) {
-            uint8_t* s = st.scales + 2 * (at / kStateBlock);
-            s[0] = (uint8_t)sm;
-            s[1] = (uint8_t)sv;
-        }
-    }
+    const uint64_t tile = (uint64_t)w.c * kSubs + blockIdx.x % kSubs, off = tb.off[w.t];
+    AdamwTensor t;
+    t.count = (int64_t)(tb.bytes[w.t] / GS);
+    if (tile * kAdamwTile >= (uint64_t)t.count) return;
+    t.at = off / GS;
+    t.p = (unsigned char*)(uintptr_t)params.get(w.t - tb.t0);
+    t.g = buffer ? buffer + off : (const unsigned char*)(uintptr_t)grads.get(w.t - tb.t0);
+    t.master = st.master + t.at;
+    t.avg = STATE == STATE_FP32 ? (void*)((float*)st.avg + t.at) : (void*)((uint8_t*)st.avg + t.at);
+    t.sq = STATE == STATE_FP32 ? (void*)((float*)st.sq + t.at) : (void*)((uint8_t*)st.sq + t.at);
+    t.scales = st.scales + 2 * (t.at / kStateBlock);
+    const int64_t back = STATE == STATE_FP32 ? (int64_t)((uintptr_t)t.avg / sizeof(float) % 64) : 0;
+    int64_t e0 = (int64_t)(tile * kAdamwTile) - back;
+    if (e0 >= 0 && e0 + (int64_t)kAdamwTile <= t.count) adamw_tile<P, G, MASTER, STATE, true>(t, e0, a, scale);
+    else adamw_tile<P, G, MASTER, STATE, false>(t, e0, a, scale);
+    // the last of the tensor's tiles (there are ceil(count / kAdamwTile)) and elements behind it
+    e0 += kAdamwTile;
+    if (STATE == STATE_FP32 && e0 < t.count && e0 + back >= t.count) adamw_tile<P, G, MASTER, STATE, false>(t, e0, a, scale);
 }
 
 // ---- 8-bit states in and out ----------------------------------------------------------------------------------------------
+
+// The part of an item that a block of the two kernels below takes: G groups of four elements of a lane, a wave 256 G in a row.
+constexpr uint32_t kEncodeGroups = 1, kDecodeGroups = 2;
+template <uint32_t G>
+struct StateTile {
+    uint64_t at;        // the lane's first element in the plan's layout; its next group is 256 elements on
+    Span n[G];
+};
+template <uint32_t G>
+__device__ __forceinline__ StateTile<G> state_tile(const AdamwTables& tb, uint32_t item_elems) {
+    constexpr uint32_t kTile = kBlock * 4 * G;
+    const uint32_t subs = item_elems / kTile;
+    const FusionItem w = tb.items[blockIdx.x / subs];
+    const uint64_t e = (uint64_t)w.c * item_elems + (blockIdx.x % subs) * kTile + (threadIdx.x >> 6) * (256 * G) + (threadIdx.x & 63u) * 4;
+    const uint64_t count = tb.bytes[w.t] >> tb.log_esize;
+    StateTile<G> s;
+    s.at = (tb.off[w.t] >> tb.log_esize) + e;
+#pragma unroll
+    for (uint32_t q = 0; q < G; q++) {
+        const uint64_t f = e + 256 * q;
+        s.n[q] = Span{ 0, f >= count ? 0 : count - f < 4 ? (int)(count - f) : 4 };
+    }
+    return s;
+}
 
 // The values of the codes, as fp32 or bfloat16 (which holds every one of them from 2^-126 up).
 template <class V>
 __global__ void __launch_bounds__(kBlock)
 state_decode_kernel(AdamwTables tb, uint32_t item_elems, const uint8_t* avg, const uint8_t* sq, const uint8_t* scales,
                     typename V::elem_t* out_avg, typename V::elem_t* out_sq) {
-    const uint32_t subs = item_elems / kOptTile;
-    const FusionItem w = tb.items[blockIdx.x / subs];
-    const uint64_t e = (uint64_t)w.c * item_elems + (blockIdx.x % subs) * kOptTile + threadIdx.x * kLaneElems;
-    const uint64_t count = tb.bytes[w.t] >> tb.log_esize;
-    if (e >= count) return;
-    const uint32_t n = count - e < kLaneElems ? (uint32_t)(count - e) : kLaneElems;
-    const uint64_t at = (tb.off[w.t] >> tb.log_esize) + e;
-    uint32_t cm[8], cv[8];
-    float m[8], v[8];
-    load_codes(avg + at, n, cm);
-    load_codes(sq + at, n, cv);
-    const uint32_t sm = scales[2 * (at / kStateBlock)], sv = scales[2 * (at / kStateBlock) + 1];
+    constexpr uint32_t G = kDecodeGroups;
+    const StateTile<G> t = state_tile<G>(tb, item_elems);
+    uint32_t cm[G], cv[G], sm[G], sv[G];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        m[i] = value_avg(cm[i], sm);
-        v[i] = value_sq(cv[i], sv);
+    for (uint32_t q = 0; q < G; q++) {
+        if (t.n[q].to == 0) continue;
+        cm[q] = load_codes<false>(avg + t.at + 256 * q, t.n[q]);
+        cv[q] = load_codes<false>(sq + t.at + 256 * q, t.n[q]);
+        sm[q] = scales[2 * (t.at / kStateBlock + q)];
+        sv[q] = scales[2 * (t.at / kStateBlock + q) + 1];
     }
-    store8<V>(out_avg + at, n, m);
-    store8<V>(out_sq + at, n, v);
+#pragma unroll
+    for (uint32_t q = 0; q < G; q++) {
+        if (t.n[q].to == 0) continue;
+        float m[4], v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            m[i] = value_avg((cm[q] >> (8 * i)) & 0xffu, sm[q]);
+            v[i] = value_sq((cv[q] >> (8 * i)) & 0xffu, sv[q]);
+        }
+        store4<V, false>(out_avg + t.at + 256 * q, t.n[q], m);
+        store4<V, false>(out_sq + t.at + 256 * q, t.n[q], v);
+    }
 }
 
 // fp32 or bfloat16 values to codes, rounded to nearest.
@@ -399,32 +498,28 @@ template <class V>
 __global__ void __launch_bounds__(kBlock)
 state_encode_kernel(AdamwTables tb, uint32_t item_elems, const typename V::elem_t* in_avg, const typename V::elem_t* in_sq, uint8_t* avg,
                     uint8_t* sq, uint8_t* scales) {
-    const uint32_t subs = item_elems / kOptTile;
-    const FusionItem w = tb.items[blockIdx.x / subs];
-    const uint64_t e = (uint64_t)w.c * item_elems + (blockIdx.x % subs) * kOptTile + threadIdx.x * kLaneElems;
-    const uint64_t count = tb.bytes[w.t] >> tb.log_esize;
-    const uint32_t n = e >= count ? 0u : count - e < kLaneElems ? (uint32_t)(count - e) : kLaneElems;
-    const uint64_t at = (tb.off[w.t] >> tb.log_esize) + e;
-    float m[8], v[8], lm = 0.0f, lv = 0.0f;
-    load8<V>(in_avg + at, n, m);
-    load8<V>(in_sq + at, n, v);
+    const StateTile<kEncodeGroups> t = state_tile<kEncodeGroups>(tb, item_elems);
+    const Span n = t.n[0];
+    float m[4], v[4], lm = 0.0f, lv = 0.0f;
+    load4<V, false>(in_avg + t.at, n, m);
+    load4<V, false>(in_sq + t.at, n, v);
 #pragma unroll
-    for (uint32_t i = 0; i < 8; i++) {
+    for (uint32_t i = 0; i < 4; i++) {
         lm = fmaxf(lm, finite_magnitude(m[i]));
         lv = fmaxf(lv, finite_magnitude(v[i]));
     }
     const uint32_t sm = scale_avg(block_max(lm)), sv = scale_sq(block_max(lv));
-    uint32_t cm[8], cv[8];
+    uint32_t cm = 0, cv = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        cm[i] = code_avg<false>(m[i], sm, 0);
-        cv[i] = code_sq<false>(v[i], sv, 0);
+    for (int i = 0; i < 4; i++) {
+        cm |= code_avg<false>(m[i], sm, 0) << (8 * i);
+        cv |= code_sq<false>(v[i], sv, 0) << (8 * i);
     }
-    store_codes(avg + at, n, cm);
-    store_codes(sq + at, n, cv);
-    if (n && (threadIdx.x & 31u) == 0) {
-        scales[2 * (at / kStateBlock)] = (uint8_t)sm;
-        scales[2 * (at / kStateBlock) + 1] = (uint8_t)sv;
+    store_codes<false>(avg + t.at, n, cm);
+    store_codes<false>(sq + t.at, n, cv);
+    if (n.to && (threadIdx.x & 63u) == 0) {
+        scales[2 * (t.at / kStateBlock)] = (uint8_t)sm;
+        scales[2 * (t.at / kStateBlock) + 1] = (uint8_t)sv;
     }
 }
 
