@@ -4,6 +4,7 @@ Every function takes device tensors (or raw device pointers) and a HIP stream an
 there is no CPU fallback: a missing library raises at load time.
 """
 import ctypes as C
+import operator
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -143,7 +144,8 @@ def _ptr(x):
 def _stream(stream):
     if stream is None:
         import torch
-        return torch.cuda.current_stream().cuda_stream
+        # what torch.cuda.current_stream().cuda_stream is, without building a Stream object (0.3 against 2.6 us)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -153,36 +155,72 @@ def _ptr_array(xs):
     return (C.c_void_p * len(xs))(*[_ptr(x) for x in xs])
 
 
+def _tensor_array(tensors):
+    """_ptr_array of what is known to be tensors."""
+    import torch
+    return (C.c_void_p * len(tensors))(*map(torch.Tensor.data_ptr, tensors))
+
+
 _TORCH_DTYPE = {INT32: "int32", INT64: "int64", FLOAT16: "float16", FLOAT32: "float32", BFLOAT16: "bfloat16"}
 _CCL_DTYPE = {v: k for k, v in _TORCH_DTYPE.items()}
+_KINDS = {}                 # torch.dtype -> (ccl dtype or -1)
 
 
-def _dtype_name(t):
-    name = str(t.dtype).replace("torch.", "")
-    if name not in _CCL_DTYPE and name != "uint8":
-        raise ValueError(f"tensors of {name} are not taken")
-    return name
+def _kind(t):
+    """The ccl datatype of a tensor's elements, -1 for one that no operator takes (the library refuses it)."""
+    k = _KINDS.get(t.dtype)
+    if k is None:
+        k = _KINDS[t.dtype] = _CCL_DTYPE.get(str(t.dtype).replace("torch.", ""), -1)
+    return k
 
 
-def _ptr_or_none(x):
-    return None if x is None else _ptr(x)
+def _refuse(what, t, wanted):
+    if t is None:
+        raise ValueError(f"{what}: missing")
+    raise ValueError(f"{what}: {wanted} is wanted, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}")
 
 
-def _check_tensors(what, tensors, dtype=None, least=0):
-    """Raises unless every tensor is contiguous memory of the current GPU, of the dtype and with at least `least` elements."""
+def _memory(what, t, dtype, least, here):
+    """Address of a contiguous tensor of the current GPU with at least `least` elements."""
+    if t is None or t.dtype is not dtype or t.numel() < least or t.get_device() != here or not t.is_contiguous():
+        _refuse(what, t, f"contiguous {dtype}, {least} elements at least, on cuda:{here}")
+    return t.data_ptr()
+
+
+def _optional(what, t, dtype, least, here):
+    return None if t is None else _memory(what, t, dtype, least, here)
+
+
+def _workspace(workspace, need, here):
+    """(address, bytes, what has to live until the call has returned) of a call's scratch memory, allocated when there is none."""
     import torch
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is None:
-            raise ValueError(f"{what}: missing")
-        if not t.is_cuda or t.device.index != here:
-            raise ValueError(f"{what}: on {t.device}, the current device is cuda:{here}")
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: not contiguous")
-        if dtype is not None and str(t.dtype) != "torch." + dtype:
-            raise ValueError(f"{what}: {t.dtype}, {dtype} is wanted")
-        if t.numel() < least:
-            raise ValueError(f"{what}: {t.numel()} elements, {least} are needed")
+    if workspace is None:
+        if not need:
+            return None, 0, None
+        workspace = torch.empty(need, dtype=torch.uint8, device=here)
+    elif workspace.get_device() != here or not workspace.is_contiguous():
+        _refuse("workspace", workspace, f"contiguous memory on cuda:{here}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def _check_tensors(what, tensors, dtype, least, here):
+    """_memory's conditions for a list, least[i] elements of the i-th.  A step over hundreds of tensors comes through here, hence
+    one C-level pass per property."""
+    import torch
+    T = torch.Tensor
+    try:
+        devices, kinds = set(map(T.get_device, tensors)), {t.dtype for t in tensors}
+        whole, sizes = all(map(T.is_contiguous, tensors)), list(map(T.numel, tensors))
+    except (TypeError, AttributeError):
+        raise ValueError(f"{what}: a tensor is missing") from None
+    if devices != {here}:
+        raise ValueError(f"{what}: not on the current device, cuda:{here}")
+    if not whole:
+        raise ValueError(f"{what}: not contiguous")
+    if kinds != {dtype}:
+        raise ValueError(f"{what}: {kinds}, {dtype} is wanted")
+    if any(map(operator.lt, sizes, least)):
+        raise ValueError(f"{what}: a tensor has fewer elements than the plan says")
 
 
 def datatype_size(dtype):
@@ -322,6 +360,7 @@ class FusionPlan:
         self.k = k
         self.dtype = dtype
         self.counts = [int(c) for c in counts]
+        self.elements = lib().mi_ccl_fusion_plan_elements(h)      # of a state or fp32 copy of the weights in the plan's layout
 
     @property
     def nbytes(self):
@@ -349,77 +388,68 @@ class FusionPlan:
 
     # ---- the optimizer step behind the reduce: gradients are the plan's tensors (a list) or its fusion buffer (one tensor) ----
 
-    @property
-    def elements(self):
-        """Elements of a state or fp32 copy of the weights in the plan's layout."""
-        return lib().mi_ccl_fusion_plan_elements(self._h)
-
-    def _gradients(self, grads):
+    def _gradients(self, grads, here):
+        import torch
+        kind = getattr(torch, _TORCH_DTYPE.get(self.dtype, "float32"))
         if isinstance(grads, (list, tuple)):
-            if len(grads) != self.k or any(t.numel() < c for t, c in zip(grads, self.counts)):
+            if len(grads) != self.k:
                 raise ValueError("the gradients are not the plan's tensors")
-            _check_tensors("gradients", grads, _TORCH_DTYPE[self.dtype])
-            return _ptr_array(grads), None
-        _check_tensors("gradients", [grads], _TORCH_DTYPE[self.dtype], self.elements)
-        return None, _ptr(grads)
+            _check_tensors("gradients", grads, kind, self.counts, here)
+            return _tensor_array(grads), None
+        return None, _memory("gradients", grads, kind, self.elements, here)
+
+    @property
+    def norm_workspace(self):
+        return lib().mi_ccl_fusion_norm_workspace(self._h)
 
     def norm(self, grads, result, multiplier=1.0, max_norm=0.0, workspace=None, stream=None):
         """result[0] = the norm of all gradients times `multiplier`, result[1] = the factor of a clipped step's gradients (two
         floats on the device).  workspace: norm_workspace bytes of device memory; allocated for the call when None."""
         import torch
-        _check_tensors("result", [result], "float32", 2)
-        if workspace is None:
-            workspace = torch.empty(self.norm_workspace, dtype=torch.uint8, device=result.device)
-        _check_tensors("workspace", [workspace])
-        lst, buf = self._gradients(grads)
-        _check(lib().mi_ccl_fusion_norm(self._h, lst, buf, multiplier, max_norm, _ptr(result), _ptr(workspace),
-                                        workspace.numel() * workspace.element_size(), _stream(stream)), "mi_ccl_fusion_norm")
-
-    @property
-    def norm_workspace(self):
-        return lib().mi_ccl_fusion_norm_workspace(self._h)
+        here = torch.cuda.current_device()
+        res = _memory("result", result, torch.float32, 2, here)
+        lst, buf = self._gradients(grads, here)
+        ws, size, _keep = _workspace(workspace, self.norm_workspace, here)
+        _check(lib().mi_ccl_fusion_norm(self._h, lst, buf, multiplier, max_norm, res, ws, size, _stream(stream)), "mi_ccl_fusion_norm")
 
     def adamw(self, params, grads, exp_avg, exp_avg_sq, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, step=1, scales=None,
               master=None, grad_scale=None, seed=None, step_ptr=None, lr_ptr=None, stream=None):
         """One AdamW step over the plan's tensors, in place.  States: float32 (32 bits) or uint8 (8 bits, with `scales`) in the
         plan's layout.  seed: not None rounds 8-bit states stochastically.  step_ptr (int64), lr_ptr and grad_scale (float32):
         one-element device tensors read by the kernel."""
-        if len(params) != self.k or any(t.numel() < c for t, c in zip(params, self.counts)):
+        import torch
+        here = torch.cuda.current_device()
+        if len(params) != self.k or params[0] is None:
             raise ValueError("the parameters are not the plan's tensors")
-        kind = _dtype_name(params[0])
-        _check_tensors("params", params, kind)
-        eight = _dtype_name(exp_avg) == "uint8"
-        _check_tensors("states", [exp_avg, exp_avg_sq], "uint8" if eight else "float32", self.elements)
-        if eight:
-            _check_tensors("scales", [scales], "uint8", 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK))
-        if master is not None:
-            _check_tensors("master", [master], "float32", self.elements)
-        for name, t, dt in (("grad_scale", grad_scale, "float32"), ("step_ptr", step_ptr, "int64"), ("lr_ptr", lr_ptr, "float32")):
-            if t is not None:
-                _check_tensors(name, [t], dt, 1)
-        lst, buf = self._gradients(grads)
+        _check_tensors("params", params, params[0].dtype, self.counts, here)
+        eight = exp_avg.dtype is torch.uint8
+        kind = torch.uint8 if eight else torch.float32
+        m, v = _memory("exp_avg", exp_avg, kind, self.elements, here), _memory("exp_avg_sq", exp_avg_sq, kind, self.elements, here)
+        sc = _memory("scales", scales, torch.uint8, 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK), here) if eight else None
         o = AdamwOptions(lr, beta1, beta2, eps, weight_decay, int(step), 0 if seed is None else int(seed), int(seed is not None),
-                         _ptr_or_none(step_ptr), _ptr_or_none(lr_ptr), _ptr_or_none(grad_scale))
-        _check(lib().mi_ccl_fusion_adamw(self._h, _CCL_DTYPE[kind], _ptr_array(params), lst, buf, STATE_8BIT if eight else STATE_FP32,
-                                         _ptr(exp_avg), _ptr(exp_avg_sq), _ptr_or_none(scales), _ptr_or_none(master), C.byref(o),
+                         _optional("step_ptr", step_ptr, torch.int64, 1, here), _optional("lr_ptr", lr_ptr, torch.float32, 1, here),
+                         _optional("grad_scale", grad_scale, torch.float32, 1, here))
+        lst, buf = self._gradients(grads, here)
+        _check(lib().mi_ccl_fusion_adamw(self._h, _kind(params[0]), _tensor_array(params), lst, buf, STATE_8BIT if eight else STATE_FP32,
+                                         m, v, sc, _optional("master", master, torch.float32, self.elements, here), C.byref(o),
                                          _stream(stream)), "mi_ccl_fusion_adamw")
 
-    def _state_tensors(self, exp_avg, exp_avg_sq, scales, values_avg, values_sq):
-        _check_tensors("states", [exp_avg, exp_avg_sq], "uint8", self.elements)
-        _check_tensors("scales", [scales], "uint8", 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK))
-        _check_tensors("values", [values_avg, values_sq], _dtype_name(values_avg), self.elements)
+    def _state_memory(self, exp_avg, exp_avg_sq, scales, values_avg, values_sq):
+        import torch
+        here = torch.cuda.current_device()
+        return (_memory("exp_avg", exp_avg, torch.uint8, self.elements, here), _memory("exp_avg_sq", exp_avg_sq, torch.uint8, self.elements, here),
+                _memory("scales", scales, torch.uint8, 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK), here),
+                _memory("values", values_avg, values_avg.dtype, self.elements, here), _memory("values", values_sq, values_avg.dtype, self.elements, here))
 
     def state_decode(self, exp_avg, exp_avg_sq, scales, values_avg, values_sq, stream=None):
         """The values of 8-bit states, float32 or bfloat16."""
-        self._state_tensors(exp_avg, exp_avg_sq, scales, values_avg, values_sq)
-        _check(lib().mi_ccl_fusion_state_decode(self._h, _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(scales), _CCL_DTYPE[_dtype_name(values_avg)],
-                                                _ptr(values_avg), _ptr(values_sq), _stream(stream)), "mi_ccl_fusion_state_decode")
+        m, v, sc, vm, vv = self._state_memory(exp_avg, exp_avg_sq, scales, values_avg, values_sq)
+        _check(lib().mi_ccl_fusion_state_decode(self._h, m, v, sc, _kind(values_avg), vm, vv, _stream(stream)), "mi_ccl_fusion_state_decode")
 
     def state_encode(self, values_avg, values_sq, exp_avg, exp_avg_sq, scales, stream=None):
         """Values (float32 or bfloat16) to 8-bit states, rounded to nearest."""
-        self._state_tensors(exp_avg, exp_avg_sq, scales, values_avg, values_sq)
-        _check(lib().mi_ccl_fusion_state_encode(self._h, _CCL_DTYPE[_dtype_name(values_avg)], _ptr(values_avg), _ptr(values_sq), _ptr(exp_avg),
-                                                _ptr(exp_avg_sq), _ptr(scales), _stream(stream)), "mi_ccl_fusion_state_encode")
+        m, v, sc, vm, vv = self._state_memory(exp_avg, exp_avg_sq, scales, values_avg, values_sq)
+        _check(lib().mi_ccl_fusion_state_encode(self._h, _kind(values_avg), vm, vv, m, v, sc, _stream(stream)), "mi_ccl_fusion_state_encode")
 
     def close(self):
         if self._h:
@@ -448,21 +478,14 @@ def fusion_reduce_static(counts, dtype, align, op, own_tensors, peers, out_tenso
 
 # ---- tokens sorted by expert, and back --------------------------------------------------------------------------------
 
-def _check_rows(what, t, hidden=None, dtype=None):
-    """(dtype, elements between rows) of a matrix of rows, whose rows are contiguous."""
-    import torch
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (hidden is not None and t.shape[1] != hidden):
-        raise ValueError(f"{what}: rows of {'contiguous' if hidden is None else hidden} elements are wanted, got {tuple(t.shape)}, strides {t.stride()}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    name = _dtype_name(t)
-    if dtype is not None and name != dtype:
-        raise ValueError(f"{what}: {name}, {dtype} is wanted")
+def _rows(what, t, hidden, dtype, here):
+    """(rows, elements from row to row, address) of a matrix whose rows are contiguous and do not overlap."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] != hidden or t.dtype is not dtype or t.get_device() != here or (hidden > 1 and stride[1] != 1) or \
+            (shape[0] > 1 and stride[0] < hidden):
+        _refuse(what, t, f"rows of {hidden} {dtype} on cuda:{here}")
     # one row, or none, has no distance to the next
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if t.shape[0] > 1 and ld < t.shape[1]:
-        raise ValueError(f"{what}: rows overlap (strides {t.stride()})")
-    return name, ld
+    return shape[0], stride[0] if shape[0] > 1 else hidden, t.data_ptr()
 
 
 def token_rows(n_tokens, top_k, n_experts, align=1, capacity=0):
@@ -483,76 +506,74 @@ def token_sort(expert_ids, n_experts, positions, counts, offsets, align=1, capac
     the same shape; -1: none); rows of each expert into counts, first rows and the end into offsets [n_experts + 1] (int32).
     workspace: token_sort_workspace bytes; allocated for the call when None."""
     import torch
-    if expert_ids.dim() != 2 or tuple(positions.shape) != tuple(expert_ids.shape):
+    here = torch.cuda.current_device()
+    shape = expert_ids.shape
+    if len(shape) != 2 or positions.shape != shape:
         raise ValueError("expert_ids and positions are [tokens, top_k]")
-    n, k = expert_ids.shape
-    _check_tensors("expert_ids", [expert_ids])
-    _check_tensors("positions", [positions], "int32")
-    _check_tensors("counts", [counts], "int32", n_experts)
-    _check_tensors("offsets", [offsets], "int32", n_experts + 1)
-    if workspace is None:
-        need = token_sort_workspace(n, k, n_experts)
-        workspace = torch.empty(need, dtype=torch.uint8, device=expert_ids.device) if need else None
-    size = 0
-    if workspace is not None:
-        _check_tensors("workspace", [workspace])
-        size = workspace.numel() * workspace.element_size()
-    _check(lib().mi_ccl_token_sort(_CCL_DTYPE.get(_dtype_name(expert_ids), -1), _ptr(expert_ids), n, k, n_experts, align, capacity,
-                                   _ptr(positions), _ptr(counts), _ptr(offsets), _ptr_or_none(workspace), size, _stream(stream)),
+    n, k = shape
+    ids = _memory("expert_ids", expert_ids, expert_ids.dtype, 0, here)
+    pos = _memory("positions", positions, torch.int32, 0, here)
+    cnt, off = _memory("counts", counts, torch.int32, n_experts, here), _memory("offsets", offsets, torch.int32, n_experts + 1, here)
+    ws, size, _keep = _workspace(workspace, token_sort_workspace(n, k, n_experts), here)
+    _check(lib().mi_ccl_token_sort(_kind(expert_ids), ids, n, k, n_experts, align, capacity, pos, cnt, off, ws, size, _stream(stream)),
            "mi_ccl_token_sort")
 
 
-def _check_segments(positions, counts, offsets, tokens):
-    _check_tensors("positions", [positions], "int32")
-    if positions.dim() != 2 or positions.shape[0] != tokens:
-        raise ValueError(f"positions: [{tokens}, top_k] is wanted, got {tuple(positions.shape)}")
-    if counts is not None:
-        _check_tensors("counts", [counts], "int32")
-        _check_tensors("offsets", [offsets], "int32", counts.numel() + 1)
+def _positions(positions, tokens, here):
+    import torch
+    shape = positions.shape
+    if len(shape) != 2 or shape[0] != tokens:
+        _refuse("positions", positions, f"[{tokens}, top_k]")
+    return shape[1], _memory("positions", positions, torch.int32, 0, here)
 
 
 def token_dispatch(x, positions, counts, offsets, out, stream=None):
     """out[positions[t, j]] = x[t]; padding rows become zero, rows behind the last expert's stay as they are."""
-    kind, ldx = _check_rows("x", x)
-    _, ldo = _check_rows("out", out, x.shape[1], kind)
-    _check_segments(positions, counts, offsets, x.shape[0])
-    _check(lib().mi_ccl_token_dispatch(_CCL_DTYPE.get(kind, -1), _ptr(x), ldx, x.shape[0], positions.shape[1], x.shape[1], _ptr(positions),
-                                       _ptr(counts), _ptr(offsets), counts.numel(), _ptr(out), ldo, out.shape[0], _stream(stream)),
+    import torch
+    here = torch.cuda.current_device()
+    hidden, experts = x.shape[-1], counts.numel()
+    n, ldx, px = _rows("x", x, hidden, x.dtype, here)
+    rows, ldo, po = _rows("out", out, hidden, x.dtype, here)
+    k, pos = _positions(positions, n, here)
+    _check(lib().mi_ccl_token_dispatch(_kind(x), px, ldx, n, k, hidden, pos, _memory("counts", counts, torch.int32, experts, here),
+                                       _memory("offsets", offsets, torch.int32, experts + 1, here), experts, po, ldo, rows, _stream(stream)),
            "mi_ccl_token_dispatch")
 
 
 def token_combine(y, positions, weights, out, stream=None):
     """out[t] = sum over j of weights[t, j] * y[positions[t, j]]; weights (float32, the shape of positions) may be None for ones."""
-    kind, ldy = _check_rows("y", y)
-    _, ldo = _check_rows("out", out, y.shape[1], kind)
-    _check_segments(positions, None, None, out.shape[0])
-    if weights is not None:
-        _check_tensors("weights", [weights], "float32", positions.numel())
-    _check(lib().mi_ccl_token_combine(_CCL_DTYPE.get(kind, -1), _ptr(y), ldy, y.shape[0], _ptr(positions), _ptr_or_none(weights),
-                                      out.shape[0], positions.shape[1], y.shape[1], _ptr(out), ldo, _stream(stream)), "mi_ccl_token_combine")
+    import torch
+    here = torch.cuda.current_device()
+    hidden = y.shape[-1]
+    rows, ldy, py = _rows("y", y, hidden, y.dtype, here)
+    n, ldo, po = _rows("out", out, hidden, y.dtype, here)
+    k, pos = _positions(positions, n, here)
+    _check(lib().mi_ccl_token_combine(_kind(y), py, ldy, rows, pos, _optional("weights", weights, torch.float32, n * k, here), n, k, hidden, po, ldo,
+                                      _stream(stream)), "mi_ccl_token_combine")
 
 
 def token_combine_backward(grad_out, y, positions, weights, counts, offsets, grad_y, grad_weights=None, stream=None):
     """The gradient of token_combine: grad_y[positions[t, j]] = weights[t, j] * grad_out[t], with padding rows zero, and unless
     None grad_weights[t, j] = <grad_out[t], y[positions[t, j]]>.  y may be None without grad_weights."""
-    kind, ldg = _check_rows("grad_out", grad_out)
-    hidden = grad_out.shape[1]
-    _, ldd = _check_rows("grad_y", grad_y, hidden, kind)
-    ldy = hidden
+    import torch
+    here = torch.cuda.current_device()
+    hidden, kind, experts = grad_out.shape[-1], grad_out.dtype, counts.numel()
+    n, ldg, pg = _rows("grad_out", grad_out, hidden, kind, here)
+    rows, ldd, pd = _rows("grad_y", grad_y, hidden, kind, here)
+    ldy, py = hidden, None
     if y is not None:
-        _, ldy = _check_rows("y", y, hidden, kind)
-        if y.shape[0] != grad_y.shape[0]:
-            raise ValueError(f"y has {y.shape[0]} rows, grad_y {grad_y.shape[0]}")
+        y_rows, ldy, py = _rows("y", y, hidden, kind, here)
+        if y_rows != rows:
+            raise ValueError(f"y has {y_rows} rows, grad_y {rows}")
     elif grad_weights is not None:
         raise ValueError("grad_weights needs y")
-    _check_segments(positions, counts, offsets, grad_out.shape[0])
-    for name, t in (("weights", weights), ("grad_weights", grad_weights)):
-        if t is not None:
-            _check_tensors(name, [t], "float32", positions.numel())
-    _check(lib().mi_ccl_token_combine_backward(_CCL_DTYPE.get(kind, -1), _ptr(grad_out), ldg, _ptr_or_none(y), ldy, grad_y.shape[0],
-                                               _ptr(positions), _ptr_or_none(weights), _ptr(counts), _ptr(offsets), counts.numel(),
-                                               grad_out.shape[0], positions.shape[1], hidden, _ptr(grad_y), ldd,
-                                               _ptr_or_none(grad_weights), _stream(stream)), "mi_ccl_token_combine_backward")
+    k, pos = _positions(positions, n, here)
+    _check(lib().mi_ccl_token_combine_backward(_kind(grad_out), pg, ldg, py, ldy, rows, pos,
+                                               _optional("weights", weights, torch.float32, n * k, here),
+                                               _memory("counts", counts, torch.int32, experts, here),
+                                               _memory("offsets", offsets, torch.int32, experts + 1, here), experts, n, k, hidden, pd, ldd,
+                                               _optional("grad_weights", grad_weights, torch.float32, n * k, here), _stream(stream)),
+           "mi_ccl_token_combine_backward")
 
 
 def token_dispatch_backward(grad_rows, positions, grad_x, stream=None):

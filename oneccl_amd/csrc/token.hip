@@ -54,17 +54,16 @@ RowShape row_shape(size_t hidden, int dtype, size_t n_tokens, int top_k, int u) 
     return s;
 }
 
-constexpr uint64_t kTokenBlockLimit = 1u << 20;     // blocks along x: a block takes more tokens beyond
-
-uint32_t token_grid(const RowShape& s) {
+// Blocks along y, which HIP limits to 65535, and along x: a block takes more tokens, or column tiles, beyond.  The blocks that
+// clear the padding come on top (1024 * kPadParts at most).
+uint32_t token_blocks(const RowShape& s) {
+    constexpr uint64_t kLimit = 65535 - (uint64_t)kSortMaxExperts * kPadParts;
     const uint64_t per_block = (kBlock / 64) >> s.log_waves;
     const uint64_t b = (s.tokens + per_block - 1) / per_block;
-    return (uint32_t)(b < kTokenBlockLimit ? b : kTokenBlockLimit);
+    return (uint32_t)(b < kLimit ? b : kLimit);
 }
-
-// blocks along y: HIP allows 65535, a block takes more column tiles beyond
-uint32_t grid_columns(const RowShape& s) {
-    return s.cols < 65535u ? s.cols : 65535u;
+uint32_t column_blocks(const RowShape& s) {
+    return s.cols < (1u << 20) ? s.cols : 1u << 20;
 }
 
 int launched(const char* name) {
@@ -90,20 +89,22 @@ int sort_launch(const I* ids, uint32_t n, uint32_t experts, uint32_t align, uint
     return launched("token_place_kernel");
 }
 
-constexpr int kDispatchU = 2;
-constexpr int kCombineU = 1;
+// Vectors of a row that a lane takes at once.  16,384 tokens x 8 rows of 8 KiB: dispatch 261 us with one, 264 with two, 278 with
+// four (a wave's stores go to eight places; more of them at once only mix more); combine 207, 203 and 205.
+constexpr int kDispatchU = 1;
+constexpr int kCombineU = 2;
 
 template <class E>
-void dispatch_launch(const RowShape& s, dim3 grid, uint32_t token_blocks, hipStream_t stream, const void* x, size_t ld_x, const int32_t* positions,
+void dispatch_launch(const RowShape& s, dim3 grid, uint32_t pad_blocks, hipStream_t stream, const void* x, size_t ld_x, const int32_t* positions,
                      const int32_t* counts, const int32_t* offsets, void* out, size_t ld_out, size_t rows) {
     hipLaunchKernelGGL((token_dispatch_kernel<E, kDispatchU>), grid, dim3(kBlock), 0, stream, (const unsigned char*)x, (uint64_t)ld_x, s,
-                       token_blocks, positions, counts, offsets, (unsigned char*)out, (uint64_t)ld_out, (uint64_t)rows);
+                       pad_blocks, positions, counts, offsets, (unsigned char*)out, (uint64_t)ld_out, (uint64_t)rows);
 }
 
 template <class V, int K>
 void combine_launch(const RowShape& s, hipStream_t stream, const void* y, size_t ld_y, size_t rows, const int32_t* positions,
                     const float* weights, void* out, size_t ld_out) {
-    hipLaunchKernelGGL((token_combine_kernel<V, kCombineU, K>), dim3(token_grid(s), grid_columns(s)), dim3(kBlock), 0, stream, (const unsigned char*)y,
+    hipLaunchKernelGGL((token_combine_kernel<V, kCombineU, K>), dim3(column_blocks(s), token_blocks(s)), dim3(kBlock), 0, stream, (const unsigned char*)y,
                        (uint64_t)ld_y, (uint64_t)rows, s, positions, weights, (unsigned char*)out, (uint64_t)ld_out);
 }
 template <class V>
@@ -117,7 +118,7 @@ void combine_by_k(const RowShape& s, hipStream_t stream, const void* y, size_t l
 
 struct BackwardArgs {
     RowShape s;
-    uint32_t block, token_blocks, grid;
+    uint32_t block, pad_blocks, grid;
     hipStream_t stream;
     const void *grad, *y;
     size_t ld_grad, ld_y, ld_grad_y, rows;
@@ -129,7 +130,7 @@ struct BackwardArgs {
 template <class V, int K, bool DOT>
 void backward_launch(const BackwardArgs& a) {
     hipLaunchKernelGGL((token_combine_backward_kernel<V, K, DOT>), dim3(a.grid), dim3(a.block), 0, a.stream, (const unsigned char*)a.grad,
-                       (uint64_t)a.ld_grad, (const unsigned char*)a.y, (uint64_t)a.ld_y, (uint64_t)a.rows, a.s, a.token_blocks, a.positions,
+                       (uint64_t)a.ld_grad, (const unsigned char*)a.y, (uint64_t)a.ld_y, (uint64_t)a.rows, a.s, a.pad_blocks, a.positions,
                        a.weights, a.counts, a.offsets, (unsigned char*)a.grad_y, (uint64_t)a.ld_grad_y, a.grad_weights);
 }
 template <class V, bool DOT>
@@ -199,12 +200,12 @@ int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens
         hidden > kMaxRows || n_tokens > kMaxRows / (uint64_t)top_k || out_rows > kMaxRows || !words_aligned(positions, counts, offsets))
         return MI_CCL_INVALID_ARGUMENTS;
     const RowShape s = row_shape(hidden, dtype, n_tokens, top_k, kDispatchU);
-    const uint32_t token_blocks = token_grid(s);
-    const dim3 grid(token_blocks + (uint32_t)n_experts, grid_columns(s));
+    const uint32_t pad_blocks = (uint32_t)n_experts * kPadParts;
+    const dim3 grid(column_blocks(s), pad_blocks + token_blocks(s));
     if (fusion_dtype_size(dtype) == 4)
-        dispatch_launch<uint32_t>(s, grid, token_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
+        dispatch_launch<uint32_t>(s, grid, pad_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
     else
-        dispatch_launch<uint16_t>(s, grid, token_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
+        dispatch_launch<uint16_t>(s, grid, pad_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
     return launched("token_dispatch_kernel");
 }
 
@@ -247,8 +248,8 @@ int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_gra
     const uint32_t most = n_tokens >= 256 ? 256 : 1024;
     a.block = 64;
     while (a.block < a.s.nvec && a.block < most) a.block <<= 1;
-    a.token_blocks = (uint32_t)(n_tokens < kTokenBlockLimit ? n_tokens : kTokenBlockLimit);
-    a.grid = a.token_blocks + (uint32_t)n_experts;
+    a.pad_blocks = (uint32_t)n_experts * kPadParts;
+    a.grid = a.pad_blocks + (uint32_t)(n_tokens < (1u << 20) ? n_tokens : 1u << 20);
     a.stream = (hipStream_t)stream;
     a.grad = grad_out;
     a.ld_grad = ld_grad;

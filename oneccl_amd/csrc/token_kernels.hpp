@@ -167,9 +167,9 @@ token_place_kernel(const I* ids, uint32_t n, uint32_t experts, uint32_t run, uin
 
 // ---- rows ---------------------------------------------------------------------------------------------------------------
 // A row of H elements: vectors of 16 bytes, then H % VEC elements.  Rows may start anywhere (H odd, a stride, a slice): the
-// vectors are loose.  1 << log_waves waves of a block take one token, and of its vectors the column tiles blockIdx.y,
-// blockIdx.y + gridDim.y, ... of (64 << log_waves) U vectors each; the elements behind the last vector belong to the last
-// tile.
+// vectors are loose.  1 << log_waves waves of a block take one token, and of its vectors the column tiles blockIdx.x,
+// blockIdx.x + gridDim.x, ... of (64 << log_waves) U vectors each, so that a row's tiles are neighbours in time; the elements
+// behind the last vector belong to the last tile.
 struct RowShape {
     uint32_t nvec, tail;        // vectors and elements behind them
     uint32_t cols;              // column tiles, at least 1
@@ -178,16 +178,19 @@ struct RowShape {
     uint64_t tokens;
 };
 
-// Clears the rows of padding behind one expert's rows.
+// Clears the rows of padding behind one expert's rows, every kPadParts-th of them; pad_blocks = experts * kPadParts blocks do
+// all.  They come first in the grid: behind the tokens' they would be what a launch waits for at its end.
+constexpr uint32_t kPadParts = 4;
 template <class E>
-__device__ __forceinline__ void clear_padding(uint32_t expert, const int32_t* counts, const int32_t* offsets, uint64_t rows,
+__device__ __forceinline__ void clear_padding(uint32_t block, const int32_t* counts, const int32_t* offsets, uint64_t rows,
                                               unsigned char* out, uint64_t ld, uint32_t nvec, uint32_t tail) {
     constexpr uint32_t VEC = 16 / sizeof(E);
+    const uint32_t expert = block / kPadParts;
     const int64_t r0 = (int64_t)offsets[expert] + counts[expert];
     int64_t r1 = offsets[expert + 1];
     if (r0 < 0) return;
     if (r1 > (int64_t)rows) r1 = (int64_t)rows;
-    for (int64_t r = r0; r < r1; r++) {
+    for (int64_t r = r0 + block % kPadParts; r < r1; r += kPadParts) {
         unsigned char* o = out + (uint64_t)r * ld * sizeof(E);
         for (uint32_t v = threadIdx.x; v < nvec; v += blockDim.x) st_loose((u32x4_u*)o + v, u32x4{ 0, 0, 0, 0 });
         for (uint32_t i = threadIdx.x; i < tail; i += blockDim.x) st_elem<E>(o, (uint64_t)nvec * VEC + i, (E)0);
@@ -204,24 +207,24 @@ __device__ __forceinline__ void load_positions(const int32_t* pos, uint32_t k, u
     }
 }
 
-// A token's columns are read once and stored to its rows.  The last gridDim.x - token_blocks blocks clear the padding, one
-// expert each.
+// A token's columns are read once and stored to its rows.
 template <class E, int U>
 __global__ void __launch_bounds__(kBlock)
-token_dispatch_kernel(const unsigned char* x, uint64_t ldx, RowShape s, uint32_t token_blocks, const int32_t* positions, const int32_t* counts,
+token_dispatch_kernel(const unsigned char* x, uint64_t ldx, RowShape s, uint32_t pad_blocks, const int32_t* positions, const int32_t* counts,
                       const int32_t* offsets, unsigned char* out, uint64_t ldo, uint64_t rows) {
     constexpr uint32_t VEC = 16 / sizeof(E);
-    if (blockIdx.x >= token_blocks) {
-        if (blockIdx.y == 0) clear_padding<E>(blockIdx.x - token_blocks, counts, offsets, rows, out, ldo, s.nvec, s.tail);
+    if (blockIdx.y < pad_blocks) {
+        if (blockIdx.x == 0) clear_padding<E>(blockIdx.y, counts, offsets, rows, out, ldo, s.nvec, s.tail);
         return;
     }
+    const uint32_t token_block = blockIdx.y - pad_blocks, token_blocks = gridDim.y - pad_blocks;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t per_block = (kBlock / 64) >> s.log_waves, width = 64u << s.log_waves;
     const uint32_t col = (wave & ((1u << s.log_waves) - 1)) * 64u + lane;
-    for (uint64_t t = (uint64_t)blockIdx.x * per_block + (wave >> s.log_waves); t < s.tokens; t += (uint64_t)token_blocks * per_block) {
+    for (uint64_t t = (uint64_t)token_block * per_block + (wave >> s.log_waves); t < s.tokens; t += (uint64_t)token_blocks * per_block) {
         const unsigned char* src = x + t * ldx * sizeof(E);
         const int32_t* pos = positions + t * s.top_k;
-        for (uint32_t c = blockIdx.y; c < s.cols; c += gridDim.y) {
+        for (uint32_t c = blockIdx.x; c < s.cols; c += gridDim.x) {
             const uint32_t v0 = c * width * U + col;
             u32x4 v[U];
 #pragma unroll
@@ -253,9 +256,9 @@ token_combine_kernel(const unsigned char* y, uint64_t ldy, uint64_t rows, RowSha
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t per_block = (kBlock / 64) >> s.log_waves, width = 64u << s.log_waves;
     const uint32_t col = (wave & ((1u << s.log_waves) - 1)) * 64u + lane;
-    for (uint64_t t = (uint64_t)blockIdx.x * per_block + (wave >> s.log_waves); t < s.tokens; t += (uint64_t)gridDim.x * per_block) {
+    for (uint64_t t = (uint64_t)blockIdx.y * per_block + (wave >> s.log_waves); t < s.tokens; t += (uint64_t)gridDim.y * per_block) {
         unsigned char* o = out + t * ldo * sizeof(E);
-        for (uint32_t c = blockIdx.y; c < s.cols; c += gridDim.y) {
+        for (uint32_t c = blockIdx.x; c < s.cols; c += gridDim.x) {
             const uint32_t v0 = c * width * U + col;
             const bool edge = c == s.cols - 1 && col < s.tail;
             float acc[U][VEC] = {}, one = 0.0f;
@@ -298,22 +301,21 @@ token_combine_kernel(const unsigned char* y, uint64_t ldy, uint64_t rows, RowSha
 }
 
 // A block takes one token: a vector of its gradient row is read once and meets the rows of up to K entries.  The dot products
-// are summed in fp32, lane by lane over the columns, then over the wave and the block in a fixed order.  The last
-// gridDim.x - token_blocks blocks clear the padding.
+// are summed in fp32, lane by lane over the columns, then over the wave and the block in a fixed order.
 template <class V, int K, bool DOT>
 __global__ void __launch_bounds__(1024)
 token_combine_backward_kernel(const unsigned char* grad, uint64_t ldg, const unsigned char* y, uint64_t ldy, uint64_t rows, RowShape s,
-                              uint32_t token_blocks, const int32_t* positions, const float* weights, const int32_t* counts,
+                              uint32_t pad_blocks, const int32_t* positions, const float* weights, const int32_t* counts,
                               const int32_t* offsets, unsigned char* grad_y, uint64_t ldd, float* grad_weights) {
     typedef typename V::elem_t E;
     constexpr int VEC = V::VEC;
-    if (blockIdx.x >= token_blocks) {
-        clear_padding<E>(blockIdx.x - token_blocks, counts, offsets, rows, grad_y, ldd, s.nvec, s.tail);
+    if (blockIdx.x < pad_blocks) {
+        clear_padding<E>(blockIdx.x, counts, offsets, rows, grad_y, ldd, s.nvec, s.tail);
         return;
     }
     __shared__ float part[16][K];
     const uint32_t tid = threadIdx.x;
-    for (uint64_t t = blockIdx.x; t < s.tokens; t += token_blocks) {
+    for (uint64_t t = blockIdx.x - pad_blocks; t < s.tokens; t += gridDim.x - pad_blocks) {
         const unsigned char* g = grad + t * ldg * sizeof(E);
         for (uint32_t j0 = 0; j0 < s.top_k; j0 += K) {
             const uint32_t k = s.top_k - j0 < (uint32_t)K ? s.top_k - j0 : (uint32_t)K;
