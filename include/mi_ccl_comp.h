@@ -308,11 +308,17 @@ int mi_ccl_token_sort(int index_dtype, const void* expert_ids, size_t n_tokens, 
                       size_t capacity, int32_t* positions, int32_t* counts, int32_t* offsets, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* Scratch memory with which mi_ccl_token_dispatch and mi_ccl_token_combine_backward go through the rows in the order of the
+ * buffer, which large calls (64 MiB of rows) gain from; 0 where they do not.  Without it (workspace NULL) they go token by token: the same
+ * results, save that the two forms add up a weight's gradient in another order. */
+int mi_ccl_token_order_workspace(int dtype, size_t n_tokens, int top_k, size_t hidden, size_t* bytes);
+
 /* out[positions[t][j]] = x[t] for every entry that has a row; rows of padding become zero, rows from offsets[n_experts] on
- * stay as they are.  A position outside [0, out_rows) is taken as -1, here and below. */
+ * stay as they are.  A position outside [0, out_rows) is taken as -1, here and below.  workspace: NULL, or
+ * mi_ccl_token_order_workspace bytes (8-byte aligned), needed by this call alone. */
 int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens, int top_k, size_t hidden,
                           const int32_t* positions, const int32_t* counts, const int32_t* offsets, int n_experts, void* out,
-                          size_t ld_out, size_t out_rows, void* stream);
+                          size_t ld_out, size_t out_rows, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out[t] = sum over j of weights[t][j] * y[positions[t][j]], accumulated in fp32 in the order of j and rounded once; a token
  * without rows gives zeros.  weights: fp32, n_tokens x top_k, or NULL for ones -- which makes it the gradient of dispatch:
@@ -322,11 +328,13 @@ int mi_ccl_token_combine(int dtype, const void* y, size_t ld_y, size_t y_rows, c
 
 /* The gradient of combine: grad_y[positions[t][j]] = weights[t][j] * grad_out[t] (rounded once; rows of padding zero, rows
  * behind the last left as they are) and, unless grad_weights is NULL, grad_weights[t][j] = the dot product of grad_out[t]
- * and y[positions[t][j]] in fp32, 0 where there is no row.  y may be NULL when grad_weights is.  grad_y has y_rows rows. */
+ * and y[positions[t][j]] in fp32, 0 where there is no row.  y may be NULL when grad_weights is.  grad_y has y_rows rows.  workspace: as
+ * for dispatch. */
 int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_grad, const void* y, size_t ld_y, size_t y_rows,
                                   const int32_t* positions, const float* weights, const int32_t* counts,
                                   const int32_t* offsets, int n_experts, size_t n_tokens, int top_k, size_t hidden, void* grad_y,
-                                  size_t ld_grad_y, float* grad_weights, void* stream);
+                                  size_t ld_grad_y, float* grad_weights, void* workspace, size_t workspace_bytes,
+                                  void* stream);
 
 /* ---- measurement aid ------------------------------------------------------------------------------ */
 
@@ -349,8 +357,8 @@ const char* mi_ccl_last_kernel(void);
  * at; default 256, i.e. one tile per block up to 65,536 blocks), "max_blocks" (cap on the grid of the streaming kernels, for callers that want CUs left free for other work; 0 = no
  * cap; while a cap is set the phased kernels, which take one block on every CU, are not chosen), "xcd_chunked" (0/1: give each of the 8 XCDs one
  * contiguous share of the buffer), "variant" (kernel form: 0 = chosen by size and shape; 1, 2, 4 = the streaming
- * kernels with that many vectors per lane where a type has them; 8 = the phased kernels at any size; a non-zero value
- * also keeps one-input calls on the general reduce kernels instead of the copy and broadcast kernels -- for tests and
+ * kernels with that many vectors per lane where a type has them; 8 = the phased kernels, and the
+ * token operators' row-ordered form, at any size; a non-zero value also keeps one-input calls on the general reduce kernels instead of the copy and broadcast kernels -- for tests and
  * measurements),
  * "phased_min_bytes" (scales the sizes from which the phased kernels are used; default 160 MB),
  * "phase_early_loads" / "phase_early_stores" (phased kernels: how many 16-byte loads / stores per lane a block still

@@ -36,7 +36,7 @@ EXPORTS = [
     "mi_ccl_fusion_reduce_static",
     "mi_ccl_fusion_plan_elements", "mi_ccl_fusion_norm_workspace", "mi_ccl_fusion_norm", "mi_ccl_fusion_adamw",
     "mi_ccl_fusion_state_decode", "mi_ccl_fusion_state_encode",
-    "mi_ccl_token_rows", "mi_ccl_token_sort_workspace", "mi_ccl_token_sort", "mi_ccl_token_dispatch", "mi_ccl_token_combine",
+    "mi_ccl_token_rows", "mi_ccl_token_sort_workspace", "mi_ccl_token_sort", "mi_ccl_token_order_workspace", "mi_ccl_token_dispatch", "mi_ccl_token_combine",
     "mi_ccl_token_combine_backward",
     "mi_ccl_probe_bandwidth", "mi_ccl_last_kernel", "mi_ccl_set_param", "mi_ccl_get_param",
 ]
@@ -112,9 +112,10 @@ def lib():
     L.mi_ccl_token_rows.argtypes = [sz, i, i, sz, sz, C.POINTER(sz)]
     L.mi_ccl_token_sort_workspace.argtypes = [sz, i, i, C.POINTER(sz)]
     L.mi_ccl_token_sort.argtypes = [i, vp, sz, i, i, sz, sz, vp, vp, vp, vp, sz, vp]
-    L.mi_ccl_token_dispatch.argtypes = [i, vp, sz, sz, i, sz, vp, vp, vp, i, vp, sz, sz, vp]
+    L.mi_ccl_token_order_workspace.argtypes = [i, sz, i, sz, C.POINTER(sz)]
+    L.mi_ccl_token_dispatch.argtypes = [i, vp, sz, sz, i, sz, vp, vp, vp, i, vp, sz, sz, vp, sz, vp]
     L.mi_ccl_token_combine.argtypes = [i, vp, sz, sz, vp, vp, sz, i, sz, vp, sz, vp]
-    L.mi_ccl_token_combine_backward.argtypes = [i, vp, sz, vp, sz, sz, vp, vp, vp, vp, i, sz, i, sz, vp, sz, vp, vp]
+    L.mi_ccl_token_combine_backward.argtypes = [i, vp, sz, vp, sz, sz, vp, vp, vp, vp, i, sz, i, sz, vp, sz, vp, vp, sz, vp]
     L.mi_ccl_probe_bandwidth.argtypes = [i, vp, i, sz, vp]
     L.mi_ccl_last_kernel.restype = C.c_char_p
     L.mi_ccl_last_kernel.argtypes = []
@@ -519,6 +520,13 @@ def token_sort(expert_ids, n_experts, positions, counts, offsets, align=1, capac
            "mi_ccl_token_sort")
 
 
+def token_order_workspace(dtype, n_tokens, top_k, hidden):
+    """Bytes of scratch memory that a large token_dispatch or token_combine_backward goes faster with."""
+    r = C.c_size_t()
+    _check(lib().mi_ccl_token_order_workspace(dtype, n_tokens, top_k, hidden, C.byref(r)), "mi_ccl_token_order_workspace")
+    return r.value
+
+
 def _positions(positions, tokens, here):
     import torch
     shape = positions.shape
@@ -527,17 +535,20 @@ def _positions(positions, tokens, here):
     return shape[1], _memory("positions", positions, torch.int32, 0, here)
 
 
-def token_dispatch(x, positions, counts, offsets, out, stream=None):
-    """out[positions[t, j]] = x[t]; padding rows become zero, rows behind the last expert's stay as they are."""
+def token_dispatch(x, positions, counts, offsets, out, workspace=None, stream=None):
+    """out[positions[t, j]] = x[t]; padding rows become zero, rows behind the last expert's stay as they are.  workspace:
+    token_order_workspace bytes; allocated for the call when None."""
     import torch
     here = torch.cuda.current_device()
     hidden, experts = x.shape[-1], counts.numel()
     n, ldx, px = _rows("x", x, hidden, x.dtype, here)
     rows, ldo, po = _rows("out", out, hidden, x.dtype, here)
     k, pos = _positions(positions, n, here)
-    _check(lib().mi_ccl_token_dispatch(_kind(x), px, ldx, n, k, hidden, pos, _memory("counts", counts, torch.int32, experts, here),
-                                       _memory("offsets", offsets, torch.int32, experts + 1, here), experts, po, ldo, rows, _stream(stream)),
-           "mi_ccl_token_dispatch")
+    kind = _kind(x)
+    ws, size, _keep = _workspace(workspace, token_order_workspace(kind, n, k, hidden), here)
+    _check(lib().mi_ccl_token_dispatch(kind, px, ldx, n, k, hidden, pos, _memory("counts", counts, torch.int32, experts, here),
+                                       _memory("offsets", offsets, torch.int32, experts + 1, here), experts, po, ldo, rows, ws, size,
+                                       _stream(stream)), "mi_ccl_token_dispatch")
 
 
 def token_combine(y, positions, weights, out, stream=None):
@@ -552,9 +563,10 @@ def token_combine(y, positions, weights, out, stream=None):
                                       _stream(stream)), "mi_ccl_token_combine")
 
 
-def token_combine_backward(grad_out, y, positions, weights, counts, offsets, grad_y, grad_weights=None, stream=None):
+def token_combine_backward(grad_out, y, positions, weights, counts, offsets, grad_y, grad_weights=None, workspace=None, stream=None):
     """The gradient of token_combine: grad_y[positions[t, j]] = weights[t, j] * grad_out[t], with padding rows zero, and unless
-    None grad_weights[t, j] = <grad_out[t], y[positions[t, j]]>.  y may be None without grad_weights."""
+    None grad_weights[t, j] = <grad_out[t], y[positions[t, j]]>.  y may be None without grad_weights.  workspace:
+    token_order_workspace bytes; allocated for the call when None."""
     import torch
     here = torch.cuda.current_device()
     hidden, kind, experts = grad_out.shape[-1], grad_out.dtype, counts.numel()
@@ -568,11 +580,13 @@ def token_combine_backward(grad_out, y, positions, weights, counts, offsets, gra
     elif grad_weights is not None:
         raise ValueError("grad_weights needs y")
     k, pos = _positions(positions, n, here)
-    _check(lib().mi_ccl_token_combine_backward(_kind(grad_out), pg, ldg, py, ldy, rows, pos,
+    dtype = _kind(grad_out)
+    ws, size, _keep = _workspace(workspace, token_order_workspace(dtype, n, k, hidden), here)
+    _check(lib().mi_ccl_token_combine_backward(dtype, pg, ldg, py, ldy, rows, pos,
                                                _optional("weights", weights, torch.float32, n * k, here),
                                                _memory("counts", counts, torch.int32, experts, here),
                                                _memory("offsets", offsets, torch.int32, experts + 1, here), experts, n, k, hidden, pd, ldd,
-                                               _optional("grad_weights", grad_weights, torch.float32, n * k, here), _stream(stream)),
+                                               _optional("grad_weights", grad_weights, torch.float32, n * k, here), ws, size, _stream(stream)),
            "mi_ccl_token_combine_backward")
 
 

@@ -119,6 +119,7 @@ void combine_by_k(const RowShape& s, hipStream_t stream, const void* y, size_t l
 struct BackwardArgs {
     RowShape s;
     uint32_t block, pad_blocks, grid;
+    int n_experts;
     hipStream_t stream;
     const void *grad, *y;
     size_t ld_grad, ld_y, ld_grad_y, rows;
@@ -146,9 +147,72 @@ void backward_by_dot(const BackwardArgs& a) {
     else backward_by_k<V, false>(a);
 }
 
+// ---- rows in the order of the buffer
+
+// Where it pays: from 64 MiB of rows, as far as HIP takes the blocks in one launch.  16,384 tokens x 8 rows of 8 KiB, dispatch
+// and combine's gradient: 184 and 377 us against 239 and 440 token by token; x 4 of 14 KiB, 8,192 tokens: 91 and 172
+// against 127 and 202; one row of 8 KiB each, 65,536 tokens: 184 and 267 against 186 and 301.  At 33 MiB (2,048 x 2 of 8 KiB) the
+// launch in front costs as much as it gains: 13 and 20 us against 11 and 19.  "variant" 8 takes it at any size.
+constexpr uint64_t kOrderBytes = 64u << 20;
+bool wants_order(int dtype, size_t n_tokens, int top_k, size_t hidden) {
+    const uint64_t entries = (uint64_t)n_tokens * (uint64_t)top_k;
+    if (entries == 0 || hidden == 0 || entries >= (1u << 22))
+        return false;
+    return entries * hidden * fusion_dtype_size(dtype) >= kOrderBytes || mi_ccl_get_param("variant") == 8;
+}
+uint32_t order_lanes(uint32_t nvec) {
+    uint32_t lanes = 64;
+    while (lanes < nvec && lanes < 512) lanes <<= 1;
+    return lanes;
+}
+// Entries per run: what keeps the run's tokens within 2 MiB, half of an XCD's L2, and leaves every XCD a run.  Measured at 8
+// choices and 8 KiB: 16,384 tokens 184 us with 2,048 entries, 190 with 1,024, 193 with 512, 201 with 256; at 4 choices and 14 KiB,
+// 8,192 tokens: 116, 93, 91, 90.
+uint32_t order_log_run(uint64_t entries, uint32_t top_k, uint64_t row_bytes) {
+    uint32_t log_run = 8;
+    while (log_run < 11 && ((2ull << log_run) / top_k) * row_bytes <= (2u << 20) && (16ull << log_run) <= entries) log_run++;
+    return log_run;
+}
+uint32_t order_blocks(uint64_t entries, uint32_t log_run) {         // eight runs at a time
+    const uint64_t runs = (entries + (1u << log_run) - 1) >> log_run;
+    return (uint32_t)(((runs + 7) / 8 * 8) << log_run);
+}
+uint32_t order_pad_blocks(int n_experts) {      // a multiple of the XCDs, which the blocks behind count on
+    return ((uint32_t)n_experts * kPadParts + 7) / 8 * 8;
+}
+int order_launch(const int32_t* positions, uint64_t entries, uint32_t log_run, size_t rows, OrderedEntry* order, hipStream_t stream) {
+    uint32_t shift = 0;
+    while (((uint64_t)(rows - 1) >> shift) >= kOrderBuckets) shift++;
+    hipLaunchKernelGGL(token_order_kernel, dim3((unsigned)((entries + (1u << log_run) - 1) >> log_run)), dim3(kOrderBlock), 0, stream, positions,
+                       entries, 1u << log_run, (uint64_t)rows, shift, order);
+    return launched("token_order_kernel");
+}
+
+template <class V, bool DOT>
+void backward_ordered(const BackwardArgs& a, const OrderedEntry* order, uint32_t log_run) {
+    const uint64_t entries = a.s.tokens * a.s.top_k;
+    const uint32_t pads = order_pad_blocks(a.n_experts);
+    hipLaunchKernelGGL((token_backward_ordered_kernel<V, DOT>), dim3(pads + order_blocks(entries, log_run)), dim3(order_lanes(a.s.nvec)), 0, a.stream,
+                       (const unsigned char*)a.grad, (uint64_t)a.ld_grad, (const unsigned char*)a.y, (uint64_t)a.ld_y, a.s.nvec, a.s.tail, a.s.top_k,
+                       entries, pads, order, log_run, a.weights, a.counts, a.offsets, (unsigned char*)a.grad_y, (uint64_t)a.ld_grad_y, (uint64_t)a.rows,
+                       a.grad_weights);
+}
+template <class V>
+void backward_ordered_by_dot(const BackwardArgs& a, const OrderedEntry* order, uint32_t log_run) {
+    if (a.grad_weights) backward_ordered<V, true>(a, order, log_run);
+    else backward_ordered<V, false>(a, order, log_run);
+}
+
 }  // namespace
 
 extern "C" {
+
+int mi_ccl_token_order_workspace(int dtype, size_t n_tokens, int top_k, size_t hidden, size_t* bytes) {
+    if (!bytes || !float_type(dtype) || top_k < 1 || n_tokens > kMaxRows / (uint64_t)top_k || hidden > kMaxRows)
+        return MI_CCL_INVALID_ARGUMENTS;
+    *bytes = wants_order(dtype, n_tokens, top_k, hidden) ? n_tokens * (size_t)top_k * sizeof(OrderedEntry) : 0;
+    return MI_CCL_SUCCESS;
+}
 
 int mi_ccl_token_rows(size_t n_tokens, int top_k, int n_experts, size_t align, size_t capacity, size_t* rows) {
     uint64_t entries = 0, r = 0;
@@ -191,7 +255,7 @@ int mi_ccl_token_sort(int index_dtype, const void* expert_ids, size_t n_tokens, 
 
 int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens, int top_k, size_t hidden, const int32_t* positions,
                           const int32_t* counts, const int32_t* offsets, int n_experts, void* out, size_t ld_out, size_t out_rows,
-                          void* stream) {
+                          void* workspace, size_t workspace_bytes, void* stream) {
     if (!float_type(dtype) || top_k < 1 || n_experts < 1 || n_experts > kSortMaxExperts)
         return MI_CCL_INVALID_ARGUMENTS;
     if (n_tokens == 0 || hidden == 0 || out_rows == 0)
@@ -199,7 +263,28 @@ int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens
     if (!row_pointer_ok(x, dtype) || !row_pointer_ok(out, dtype) || !positions || !counts || !offsets || ld_x < hidden || ld_out < hidden ||
         hidden > kMaxRows || n_tokens > kMaxRows / (uint64_t)top_k || out_rows > kMaxRows || !words_aligned(positions, counts, offsets))
         return MI_CCL_INVALID_ARGUMENTS;
+    if ((uintptr_t)workspace % sizeof(OrderedEntry))
+        return MI_CCL_INVALID_ARGUMENTS;
     const RowShape s = row_shape(hidden, dtype, n_tokens, top_k, kDispatchU);
+    const uint64_t entries = (uint64_t)n_tokens * (uint64_t)top_k;
+    if (workspace && workspace_bytes / sizeof(OrderedEntry) >= entries && wants_order(dtype, n_tokens, top_k, hidden)) {
+        OrderedEntry* order = (OrderedEntry*)workspace;
+        const uint32_t log_run = order_log_run(entries, s.top_k, hidden * fusion_dtype_size(dtype));
+        const int rc = order_launch(positions, entries, log_run, out_rows, order, (hipStream_t)stream);
+        if (rc != MI_CCL_SUCCESS)
+            return rc;
+        const uint32_t pads = order_pad_blocks(n_experts);
+        const dim3 grid(pads + order_blocks(entries, log_run)), block(order_lanes(s.nvec));
+        if (fusion_dtype_size(dtype) == 4)
+            hipLaunchKernelGGL((token_dispatch_ordered_kernel<uint32_t>), grid, block, 0, (hipStream_t)stream, (const unsigned char*)x, (uint64_t)ld_x,
+                               s.nvec, s.tail, s.top_k, entries, pads, (const OrderedEntry*)order, log_run, counts, offsets, (unsigned char*)out,
+                               (uint64_t)ld_out, (uint64_t)out_rows);
+        else
+            hipLaunchKernelGGL((token_dispatch_ordered_kernel<uint16_t>), grid, block, 0, (hipStream_t)stream, (const unsigned char*)x, (uint64_t)ld_x,
+                               s.nvec, s.tail, s.top_k, entries, pads, (const OrderedEntry*)order, log_run, counts, offsets, (unsigned char*)out,
+                               (uint64_t)ld_out, (uint64_t)out_rows);
+        return launched("token_dispatch_ordered_kernel");
+    }
     const uint32_t pad_blocks = (uint32_t)n_experts * kPadParts;
     const dim3 grid(column_blocks(s), pad_blocks + token_blocks(s));
     if (fusion_dtype_size(dtype) == 4)
@@ -228,13 +313,13 @@ int mi_ccl_token_combine(int dtype, const void* y, size_t ld_y, size_t y_rows, c
 int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_grad, const void* y, size_t ld_y, size_t y_rows,
                                   const int32_t* positions, const float* weights, const int32_t* counts, const int32_t* offsets,
                                   int n_experts, size_t n_tokens, int top_k, size_t hidden, void* grad_y, size_t ld_grad_y,
-                                  float* grad_weights, void* stream) {
+                                  float* grad_weights, void* workspace, size_t workspace_bytes, void* stream) {
     if (!float_type(dtype) || top_k < 1 || n_experts < 1 || n_experts > kSortMaxExperts)
         return MI_CCL_INVALID_ARGUMENTS;
     if (n_tokens == 0)
         return MI_CCL_SUCCESS;
     if (!positions || !counts || !offsets || hidden > kMaxRows || n_tokens > kMaxRows / (uint64_t)top_k || y_rows > kMaxRows ||
-        !words_aligned(positions, weights, counts, offsets, grad_weights))
+        !words_aligned(positions, weights, counts, offsets, grad_weights) || (uintptr_t)workspace % sizeof(OrderedEntry))
         return MI_CCL_INVALID_ARGUMENTS;
     if (hidden && (!row_pointer_ok(grad_out, dtype) || ld_grad < hidden))
         return MI_CCL_INVALID_ARGUMENTS;
@@ -249,6 +334,7 @@ int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_gra
     const uint32_t most = n_tokens >= 256 ? 512 : 1024;
     a.block = 64;
     while (a.block < a.s.nvec && a.block < most) a.block <<= 1;
+    a.n_experts = n_experts;
     a.pad_blocks = (uint32_t)n_experts * kPadParts;
     a.grid = a.pad_blocks + (uint32_t)(n_tokens < (1u << 20) ? n_tokens : 1u << 20);
     a.stream = (hipStream_t)stream;
@@ -264,6 +350,17 @@ int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_gra
     a.grad_y = grad_y;
     a.ld_grad_y = ld_grad_y;
     a.grad_weights = grad_weights;
+    const uint64_t entries = (uint64_t)n_tokens * (uint64_t)top_k;
+    if (y_rows && workspace && workspace_bytes / sizeof(OrderedEntry) >= entries && wants_order(dtype, n_tokens, top_k, hidden)) {
+        const uint32_t log_run = order_log_run(entries, a.s.top_k, hidden * fusion_dtype_size(dtype));
+        const int rc = order_launch(positions, entries, log_run, y_rows, (OrderedEntry*)workspace, (hipStream_t)stream);
+        if (rc != MI_CCL_SUCCESS)
+            return rc;
+        if (dtype == MI_CCL_FLOAT32) backward_ordered_by_dot<F32Vec>(a, (const OrderedEntry*)workspace, log_run);
+        else if (dtype == MI_CCL_BFLOAT16) backward_ordered_by_dot<Bf16Vec>(a, (const OrderedEntry*)workspace, log_run);
+        else backward_ordered_by_dot<Fp16Vec>(a, (const OrderedEntry*)workspace, log_run);
+        return launched("token_backward_ordered_kernel");
+    }
     if (dtype == MI_CCL_FLOAT32) backward_by_dot<F32Vec>(a);
     else if (dtype == MI_CCL_BFLOAT16) backward_by_dot<Bf16Vec>(a);
     else backward_by_dot<Fp16Vec>(a);

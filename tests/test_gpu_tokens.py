@@ -110,7 +110,17 @@ def half_step(kind, x):
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("shape", SHAPES)
 @pytest.mark.parametrize("pad,shift", [(0, 0), (3, 1)])
-def test_dispatch_combine_and_gradients(comp, shape, kind, pad, shift):
+@pytest.mark.parametrize("ordered", [False, True])
+def test_dispatch_combine_and_gradients(comp, shape, kind, pad, shift, ordered):
+    """Token by token, and in the order of the rows, which large calls take (forced here by the variant knob)."""
+    comp.set_param("variant", 8 if ordered else 0)
+    try:
+        run_dispatch_combine_and_gradients(comp, shape, kind, pad, shift, ordered)
+    finally:
+        comp.set_param("variant", 0)
+
+
+def run_dispatch_combine_and_gradients(comp, shape, kind, pad, shift, ordered):
     import torch
     tokens, k, experts, hidden, align, dropped = shape
     rng = np.random.default_rng(hidden)
@@ -123,6 +133,7 @@ def test_dispatch_combine_and_gradients(comp, shape, kind, pad, shift):
     before = out.clone()
     guard = out_all.clone()
     comp.token_dispatch(x, pos, counts, offsets, out)
+    assert comp.last_kernel() == ("token_dispatch_ordered_kernel" if ordered else "token_dispatch_kernel")
     want = host(before)
     want[:ho[-1]] = 0
     for t in range(tokens):
@@ -156,6 +167,7 @@ def test_dispatch_combine_and_gradients(comp, shape, kind, pad, shift):
         keep, guard = gy.clone(), gy_all.clone()
         gw = torch.full((tokens, k), 7.0, device="cuda")
         comp.token_combine_backward(g, y, pos, w, counts, offsets, gy, gw)
+        assert comp.last_kernel() == ("token_backward_ordered_kernel" if ordered else "token_combine_backward_kernel")
         ref, tol = host(keep), np.zeros((rows, hidden))
         ref[:ho[-1]] = 0
         for t in range(tokens):
@@ -179,8 +191,17 @@ def test_dispatch_combine_and_gradients(comp, shape, kind, pad, shift):
             assert torch.equal(gx, (lambda r: (comp.token_combine(y, pos, None, r), r)[1])(torch.zeros_like(gx)))
 
 
-def test_one_expert_twice_and_positions_outside(comp):
+@pytest.mark.parametrize("variant", [0, 8])
+def test_one_expert_twice_and_positions_outside(comp, variant):
     """A token that names an expert twice has two rows there; positions outside the buffer count as none."""
+    comp.set_param("variant", variant)
+    try:
+        run_one_expert_twice_and_positions_outside(comp)
+    finally:
+        comp.set_param("variant", 0)
+
+
+def run_one_expert_twice_and_positions_outside(comp):
     import torch
     ids = np.array([[2, 2], [2, 0]], np.int64)
     pos, counts, offsets = sort(comp, ids, 3)
@@ -202,6 +223,36 @@ def test_one_expert_twice_and_positions_outside(comp):
     # no rows at all
     comp.token_combine(torch.zeros(0, 5, device="cuda"), bad, None, res)
     assert not res.any()
+
+
+@pytest.mark.parametrize("tokens,k,experts,hidden,kind", [(6007, 6, 40, 1000, "bfloat16"), (70001, 1, 8, 257, "float32")])
+def test_many_runs_in_order_equal_token_by_token(comp, tokens, k, experts, hidden, kind):
+    """From 64 MiB of rows the order is taken by itself (runs on every XCD, a last run that is not full): the same rows as without
+    scratch memory, to the bit; the weights' gradients within the bound of their sums."""
+    import torch
+    rng = np.random.default_rng(tokens)
+    ids = make_ids(rng, tokens, k, experts, 0.05)
+    pos, counts, offsets = sort(comp, ids, experts, 8)
+    rows = comp.token_rows(tokens, k, experts, 8)
+    t = getattr(torch, kind)
+    x, y = (torch.randn(n, hidden, device="cuda").to(t) for n in (tokens, rows))
+    w = torch.randn(tokens, k, device="cuda")
+    assert comp.token_order_workspace(comp.FLOAT32 if kind == "float32" else comp.BFLOAT16, tokens, k, hidden) == 8 * tokens * k
+    none = torch.zeros(1, dtype=torch.int64, device="cuda")
+    outs = [(torch.full((rows, hidden), 3.0, device="cuda", dtype=t), torch.full((rows, hidden), 3.0, device="cuda", dtype=t), torch.zeros(tokens, k, device="cuda"))
+            for _ in range(2)]
+    for (out, gy, gw), ws, name in zip(outs, (None, none), ("ordered_kernel", "_kernel")):
+        comp.token_dispatch(x, pos, counts, offsets, out, workspace=ws)
+        assert comp.last_kernel().endswith(name)
+        comp.token_combine_backward(x, y, pos, w, counts, offsets, gy, gw, workspace=ws)
+        assert comp.last_kernel().endswith(name)
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    some = pos >= 0
+    sums = torch.zeros(tokens, k, device="cuda", dtype=torch.float64)
+    for j in range(k):
+        at = pos[:, j].long().clamp(min=0)
+        sums[:, j] = (x.double() * y[at].double()).abs().sum(1) * some[:, j]
+    assert ((outs[0][2] - outs[1][2]).abs().double() <= 2 * hidden * U32 * sums).all()
 
 
 def test_what_is_not_finite_stays_where_it_is(comp):

@@ -42,12 +42,13 @@ def test_sort_refusals():
 
 def test_dispatch_refusals():
     f = c.lib().mi_ccl_token_dispatch
-    ok = dict(dt=c.BFLOAT16, x=A, ldx=8, n=3, k=2, h=8, pos=A, cnt=A, off=A, e=4, out=A, ldo=8, rows=6)
+    ok = dict(dt=c.BFLOAT16, x=A, ldx=8, n=3, k=2, h=8, pos=A, cnt=A, off=A, e=4, out=A, ldo=8, rows=6, ws=None, wb=0)
 
     def call(**kw):
         d = dict(ok, **kw)
-        return f(d["dt"], d["x"], d["ldx"], d["n"], d["k"], d["h"], d["pos"], d["cnt"], d["off"], d["e"], d["out"], d["ldo"], d["rows"], None)
-    for kw in (dict(dt=c.INT8), dict(dt=c.FLOAT64), dict(x=None), dict(x=A + 1), dict(dt=c.FLOAT32, out=A + 2), dict(ldx=7), dict(ldo=7), dict(k=0),
+        return f(d["dt"], d["x"], d["ldx"], d["n"], d["k"], d["h"], d["pos"], d["cnt"], d["off"], d["e"], d["out"], d["ldo"], d["rows"], d["ws"], d["wb"],
+                 None)
+    for kw in (dict(ws=A + 4, wb=1 << 20), dict(dt=c.INT8), dict(dt=c.FLOAT64), dict(x=None), dict(x=A + 1), dict(dt=c.FLOAT32, out=A + 2), dict(ldx=7), dict(ldo=7), dict(k=0),
                dict(pos=None), dict(cnt=None), dict(off=None), dict(e=0), dict(e=2000), dict(out=None), dict(rows=1 << 31), dict(n=1 << 31)):
         assert call(**kw) == BAD, kw
     for kw in (dict(n=0, x=None, pos=None), dict(h=0, x=None), dict(rows=0, out=None)):
@@ -70,14 +71,15 @@ def test_combine_refusals():
 
 def test_combine_backward_refusals():
     f = c.lib().mi_ccl_token_combine_backward
-    ok = dict(dt=c.FLOAT32, g=A, ldg=8, y=A, ldy=8, rows=6, pos=A, w=A, cnt=A, off=A, e=4, n=3, k=2, h=8, gy=A, ldd=8, gw=A)
+    ok = dict(dt=c.FLOAT32, g=A, ldg=8, y=A, ldy=8, rows=6, pos=A, w=A, cnt=A, off=A, e=4, n=3, k=2, h=8, gy=A, ldd=8, gw=A, ws=None)
 
     def call(**kw):
         d = dict(ok, **kw)
         return f(d["dt"], d["g"], d["ldg"], d["y"], d["ldy"], d["rows"], d["pos"], d["w"], d["cnt"], d["off"], d["e"], d["n"], d["k"], d["h"], d["gy"],
-                 d["ldd"], d["gw"], None)
+                 d["ldd"], d["gw"], d["ws"], 1 << 20, None)
     for kw in (dict(dt=c.INT32), dict(g=None), dict(g=A + 2), dict(ldg=7), dict(y=None), dict(ldy=7), dict(pos=None), dict(cnt=None), dict(off=None),
-               dict(gy=None), dict(gy=A + 2), dict(ldd=7), dict(e=0), dict(k=0), dict(n=1 << 31), dict(rows=1 << 31), dict(gw=A + 2), dict(w=A + 1)):
+               dict(gy=None), dict(gy=A + 2), dict(ldd=7), dict(e=0), dict(k=0), dict(n=1 << 31), dict(rows=1 << 31), dict(gw=A + 2), dict(w=A + 1),
+               dict(ws=A + 4)):
         assert call(**kw) == BAD, kw
     assert call(n=0, g=None, y=None, pos=None) == OK
     assert call(gw=None, h=0, g=None) == OK
