@@ -71,7 +71,7 @@ struct AdamwLaunch {
 };
 template <class P, class G, bool MASTER, int STATE>
 hipError_t adamw_launch(const AdamwLaunch& a) {
-    hipLaunchKernelGGL((fusion_adamw_kernel<P, G, MASTER, STATE>), dim3(a.blocks), dim3(AdamwShape<STATE>::block), 0, a.stream, *a.params, *a.grads, a.buffer, a.tb,
+    hipLaunchKernelGGL((fusion_adamw_kernel<P, G, MASTER, STATE>), dim3(a.blocks), dim3(kAdamwBlock), 0, a.stream, *a.params, *a.grads, a.buffer, a.tb,
                        a.st, a.sc);
     return hipGetLastError();
 }
