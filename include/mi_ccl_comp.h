@@ -18,7 +18,7 @@
  *   - Return value: a ccl::status number (src/internal_types.hpp:29-37): 0 success, 1 out_of_resource,
  *     2 invalid_arguments, 3 runtime_error.  Nothing here throws or terminates the process; count == 0
  *     succeeds without touching any pointer (comp.cpp:132-134, :61-63).
- *   - Results are bit-identical to the reference CPU reduction on the same inputs (integers wrap;
+ *   - Results of what has a counterpart in the reference are bit-identical to the reference CPU reduction on the same inputs (integers wrap;
  *     one IEEE operation per pair in input order, no FMA; min/max return the same operand as the
  *     reference on ties and NaNs).  NaN results of sum and prod are the x86 ones too: a NaN operand comes back with
  *     its quiet bit set, an invalid operation (Inf - Inf, 0 x Inf) gives the negative default NaN; only when both
@@ -248,15 +248,15 @@ int mi_ccl_fusion_norm(mi_ccl_fusion_plan* plan, const void* const* grads, const
  *                      exponent, 3 of mantissa (e4m3, largest 448); exp_avg_sq: 4 bits of exponent, 4 of mantissa, no sign
  *                      (code c < 16 is c, others (16 + c % 16) * 2^(c / 16 - 1); 255 is NaN).  scales: two bytes per block of
  *                      the layout (exp_avg's, exp_avg_sq's), 2 * ceil(elements / 256) in all; a code's value is multiplied
- *                      with 2^(byte - 127).  An exp_avg_sq above zero is never rounded to zero.  A fresh state is all zeros:
- *                      zero codes with zero scale bytes. */
+ *                      with 2^(byte - 127), bytes run from 1 to 247.  An exp_avg_sq above zero is never rounded to zero.
+ *                      A fresh state is all zeros, scales included. */
 enum mi_ccl_state_format { MI_CCL_STATE_FP32 = 0, MI_CCL_STATE_8BIT = 1 };
 #define MI_CCL_STATE_BLOCK 256
 size_t mi_ccl_fusion_plan_elements(const mi_ccl_fusion_plan* plan);
 
 typedef struct mi_ccl_adamw_options {
     double lr, beta1, beta2, eps, weight_decay;
-    int64_t step;               /* this step's number, from 1 */
+    int64_t step;               /* this step's number, from 1 (the one behind step_ptr too) */
     uint64_t seed;              /* of the random bits of stochastic rounding, together with the step's number */
     int stochastic;             /* 8-bit states: 0 = rounded to nearest, 1 = up with the probability of what is cut off */
     const int64_t* step_ptr;    /* device, or NULL: read in place of `step` (a step captured into a graph) */
@@ -299,7 +299,7 @@ int mi_ccl_fusion_state_encode(mi_ccl_fusion_plan* plan, int value_dtype, const 
 /* Most rows that the sorted buffer can take: min(entries, capacity * n_experts) + padding.  Host arithmetic only. */
 int mi_ccl_token_rows(size_t n_tokens, int top_k, int n_experts, size_t align, size_t capacity, size_t* rows);
 
-/* expert_ids: n_tokens x top_k ids, INT32 or INT64 (index_dtype).  Writes positions[n_tokens x top_k], the row of each
+/* expert_ids: n_tokens x top_k ids, row after row, INT32 or INT64 (index_dtype).  Writes positions[n_tokens x top_k], the row of each
  * entry in the sorted buffer or -1; counts[n_experts], the entries that each expert keeps; offsets[n_experts + 1], the first
  * row of each expert and the end of the last.  workspace: mi_ccl_token_sort_workspace bytes (0 for up to 8,192 entries),
  * needed by this call alone.  With n_tokens == 0 counts and offsets become zero. */
@@ -315,7 +315,8 @@ int mi_ccl_token_order_workspace(int dtype, size_t n_tokens, int top_k, size_t h
 
 /* out[positions[t][j]] = x[t] for every entry that has a row; rows of padding become zero, rows from offsets[n_experts] on
  * stay as they are.  A position outside [0, out_rows) is taken as -1, here and below.  workspace: NULL, or
- * mi_ccl_token_order_workspace bytes (8-byte aligned), needed by this call alone. */
+ * mi_ccl_token_order_workspace bytes (8-byte aligned), needed by this call alone.  out must not overlap x; counts and
+ * offsets are those of the sort that made the positions, with its n_experts. */
 int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens, int top_k, size_t hidden,
                           const int32_t* positions, const int32_t* counts, const int32_t* offsets, int n_experts, void* out,
                           size_t ld_out, size_t out_rows, void* workspace, size_t workspace_bytes, void* stream);
@@ -328,8 +329,8 @@ int mi_ccl_token_combine(int dtype, const void* y, size_t ld_y, size_t y_rows, c
 
 /* The gradient of combine: grad_y[positions[t][j]] = weights[t][j] * grad_out[t] (rounded once; rows of padding zero, rows
  * behind the last left as they are) and, unless grad_weights is NULL, grad_weights[t][j] = the dot product of grad_out[t]
- * and y[positions[t][j]] in fp32, 0 where there is no row.  y may be NULL when grad_weights is.  grad_y has y_rows rows.  workspace: as
- * for dispatch. */
+ * and y[positions[t][j]] in fp32, 0 where there is no row.  y may be NULL when grad_weights is.  grad_y has y_rows rows and
+ * overlaps neither grad_out nor y.  workspace: as for dispatch. */
 int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_grad, const void* y, size_t ld_y, size_t y_rows,
                                   const int32_t* positions, const float* weights, const int32_t* counts,
                                   const int32_t* offsets, int n_experts, size_t n_tokens, int top_k, size_t hidden, void* grad_y,

@@ -152,6 +152,11 @@ def _stream(stream):
     return stream.cuda_stream
 
 
+def _device():
+    import torch
+    return torch.cuda.current_device()
+
+
 def _ptr_array(xs):
     return (C.c_void_p * len(xs))(*[_ptr(x) for x in xs])
 
@@ -192,13 +197,20 @@ def _optional(what, t, dtype, least, here):
     return None if t is None else _memory(what, t, dtype, least, here)
 
 
-def _workspace(workspace, need, here):
-    """(address, bytes, what has to live until the call has returned) of a call's scratch memory, allocated when there is none."""
+def _workspace(workspace, need, here, stream):
+    """(address, bytes, what has to live until the call has returned) of a call's scratch memory, allocated when there is none:
+    from the pool of the stream that the call runs on, whose order is what makes the memory free for it and, later, for others."""
     import torch
     if workspace is None:
         if not need:
             return None, 0, None
-        workspace = torch.empty(need, dtype=torch.uint8, device=here)
+        if stream is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=here)
+        else:
+            if isinstance(stream, int):
+                stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(need, dtype=torch.uint8, device=here)
     elif workspace.get_device() != here or not workspace.is_contiguous():
         _refuse("workspace", workspace, f"contiguous memory on cuda:{here}")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
@@ -361,6 +373,7 @@ class FusionPlan:
         self.k = k
         self.dtype = dtype
         self.counts = [int(c) for c in counts]
+        self._here = _device()              # the GPU that holds the plan's table
         self.elements = lib().mi_ccl_fusion_plan_elements(h)      # of a state or fp32 copy of the weights in the plan's layout
 
     @property
@@ -389,6 +402,12 @@ class FusionPlan:
 
     # ---- the optimizer step behind the reduce: gradients are the plan's tensors (a list) or its fusion buffer (one tensor) ----
 
+    def _device(self):
+        here = _device()
+        if here != self._here:
+            raise ValueError(f"the plan was made on cuda:{self._here}, the current device is cuda:{here}")
+        return here
+
     def _gradients(self, grads, here):
         import torch
         kind = getattr(torch, _TORCH_DTYPE.get(self.dtype, "float32"))
@@ -407,10 +426,10 @@ class FusionPlan:
         """result[0] = the norm of all gradients times `multiplier`, result[1] = the factor of a clipped step's gradients (two
         floats on the device).  workspace: norm_workspace bytes of device memory; allocated for the call when None."""
         import torch
-        here = torch.cuda.current_device()
+        here = self._device()
         res = _memory("result", result, torch.float32, 2, here)
         lst, buf = self._gradients(grads, here)
-        ws, size, _keep = _workspace(workspace, self.norm_workspace, here)
+        ws, size, _keep = _workspace(workspace, self.norm_workspace, here, stream)
         _check(lib().mi_ccl_fusion_norm(self._h, lst, buf, multiplier, max_norm, res, ws, size, _stream(stream)), "mi_ccl_fusion_norm")
 
     def adamw(self, params, grads, exp_avg, exp_avg_sq, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, step=1, scales=None,
@@ -419,7 +438,7 @@ class FusionPlan:
         plan's layout.  seed: not None rounds 8-bit states stochastically.  step_ptr (int64), lr_ptr and grad_scale (float32):
         one-element device tensors read by the kernel."""
         import torch
-        here = torch.cuda.current_device()
+        here = self._device()
         if len(params) != self.k or params[0] is None:
             raise ValueError("the parameters are not the plan's tensors")
         _check_tensors("params", params, params[0].dtype, self.counts, here)
@@ -437,7 +456,7 @@ class FusionPlan:
 
     def _state_memory(self, exp_avg, exp_avg_sq, scales, values_avg, values_sq):
         import torch
-        here = torch.cuda.current_device()
+        here = self._device()
         return (_memory("exp_avg", exp_avg, torch.uint8, self.elements, here), _memory("exp_avg_sq", exp_avg_sq, torch.uint8, self.elements, here),
                 _memory("scales", scales, torch.uint8, 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK), here),
                 _memory("values", values_avg, values_avg.dtype, self.elements, here), _memory("values", values_sq, values_avg.dtype, self.elements, here))
@@ -507,7 +526,7 @@ def token_sort(expert_ids, n_experts, positions, counts, offsets, align=1, capac
     the same shape; -1: none); rows of each expert into counts, first rows and the end into offsets [n_experts + 1] (int32).
     workspace: token_sort_workspace bytes; allocated for the call when None."""
     import torch
-    here = torch.cuda.current_device()
+    here = _device()
     shape = expert_ids.shape
     if len(shape) != 2 or positions.shape != shape:
         raise ValueError("expert_ids and positions are [tokens, top_k]")
@@ -515,7 +534,7 @@ def token_sort(expert_ids, n_experts, positions, counts, offsets, align=1, capac
     ids = _memory("expert_ids", expert_ids, expert_ids.dtype, 0, here)
     pos = _memory("positions", positions, torch.int32, 0, here)
     cnt, off = _memory("counts", counts, torch.int32, n_experts, here), _memory("offsets", offsets, torch.int32, n_experts + 1, here)
-    ws, size, _keep = _workspace(workspace, token_sort_workspace(n, k, n_experts), here)
+    ws, size, _keep = _workspace(workspace, token_sort_workspace(n, k, n_experts), here, stream)
     _check(lib().mi_ccl_token_sort(_kind(expert_ids), ids, n, k, n_experts, align, capacity, pos, cnt, off, ws, size, _stream(stream)),
            "mi_ccl_token_sort")
 
@@ -539,13 +558,13 @@ def token_dispatch(x, positions, counts, offsets, out, workspace=None, stream=No
     """out[positions[t, j]] = x[t]; padding rows become zero, rows behind the last expert's stay as they are.  workspace:
     token_order_workspace bytes; allocated for the call when None."""
     import torch
-    here = torch.cuda.current_device()
+    here = _device()
     hidden, experts = x.shape[-1], counts.numel()
     n, ldx, px = _rows("x", x, hidden, x.dtype, here)
     rows, ldo, po = _rows("out", out, hidden, x.dtype, here)
     k, pos = _positions(positions, n, here)
     kind = _kind(x)
-    ws, size, _keep = _workspace(workspace, token_order_workspace(kind, n, k, hidden), here)
+    ws, size, _keep = _workspace(workspace, token_order_workspace(kind, n, k, hidden), here, stream)
     _check(lib().mi_ccl_token_dispatch(kind, px, ldx, n, k, hidden, pos, _memory("counts", counts, torch.int32, experts, here),
                                        _memory("offsets", offsets, torch.int32, experts + 1, here), experts, po, ldo, rows, ws, size,
                                        _stream(stream)), "mi_ccl_token_dispatch")
@@ -554,7 +573,7 @@ def token_dispatch(x, positions, counts, offsets, out, workspace=None, stream=No
 def token_combine(y, positions, weights, out, stream=None):
     """out[t] = sum over j of weights[t, j] * y[positions[t, j]]; weights (float32, the shape of positions) may be None for ones."""
     import torch
-    here = torch.cuda.current_device()
+    here = _device()
     hidden = y.shape[-1]
     rows, ldy, py = _rows("y", y, hidden, y.dtype, here)
     n, ldo, po = _rows("out", out, hidden, y.dtype, here)
@@ -568,7 +587,7 @@ def token_combine_backward(grad_out, y, positions, weights, counts, offsets, gra
     None grad_weights[t, j] = <grad_out[t], y[positions[t, j]]>.  y may be None without grad_weights.  workspace:
     token_order_workspace bytes; allocated for the call when None."""
     import torch
-    here = torch.cuda.current_device()
+    here = _device()
     hidden, kind, experts = grad_out.shape[-1], grad_out.dtype, counts.numel()
     n, ldg, pg = _rows("grad_out", grad_out, hidden, kind, here)
     rows, ldd, pd = _rows("grad_y", grad_y, hidden, kind, here)
@@ -581,7 +600,7 @@ def token_combine_backward(grad_out, y, positions, weights, counts, offsets, gra
         raise ValueError("grad_weights needs y")
     k, pos = _positions(positions, n, here)
     dtype = _kind(grad_out)
-    ws, size, _keep = _workspace(workspace, token_order_workspace(dtype, n, k, hidden), here)
+    ws, size, _keep = _workspace(workspace, token_order_workspace(dtype, n, k, hidden), here, stream)
     _check(lib().mi_ccl_token_combine_backward(dtype, pg, ldg, py, ldy, rows, pos,
                                                _optional("weights", weights, torch.float32, n * k, here),
                                                _memory("counts", counts, torch.int32, experts, here),

@@ -233,3 +233,55 @@ def test_a_stream_that_is_not_the_current_one(comp):
     comp.token_dispatch(x, pos, counts, offsets, out, stream=st)
     st.synchronize()
     assert (out == 3).all()
+
+
+@pytest.mark.parametrize("variant", [0, 8])
+def test_scratch_memory_that_the_binding_allocates_in_a_graph_and_on_a_side_stream(comp, variant):
+    """Sort, dispatch, gradients and norm with their scratch memory from the call itself: captured (the graph's own pool keeps it),
+    replayed between eager work, and on a stream that is not the current one while the current one allocates and writes."""
+    import torch
+    rng = np.random.default_rng(4)
+    tokens, k, experts, hidden = 9001, 2, 33, 40                       # more entries than one block sorts
+    ids = torch.from_numpy(rng.integers(-1, experts, (tokens, k)).astype(np.int32)).cuda()
+    x, w = torch.randn(tokens, hidden, device="cuda").bfloat16(), torch.rand(tokens, k, device="cuda")
+    rows = comp.token_rows(tokens, k, experts, 8)
+    plan = comp.FusionPlan([100000, 77777], comp.FLOAT32, 1)
+    grads = torch.randn(plan.elements, device="cuda")
+
+    def buffers():
+        return dict(pos=torch.zeros(tokens, k, dtype=torch.int32, device="cuda"), counts=torch.zeros(experts, dtype=torch.int32, device="cuda"),
+                    offsets=torch.zeros(experts + 1, dtype=torch.int32, device="cuda"), out=torch.zeros(rows, hidden, device="cuda").bfloat16(),
+                    gy=torch.zeros(rows, hidden, device="cuda").bfloat16(), gw=torch.zeros(tokens, k, device="cuda"), res=torch.zeros(2, device="cuda"))
+
+    def run(b, stream=None):
+        comp.token_sort(ids, experts, b["pos"], b["counts"], b["offsets"], align=8, stream=stream)
+        comp.token_dispatch(x, b["pos"], b["counts"], b["offsets"], b["out"], stream=stream)
+        comp.token_combine_backward(x, b["out"], b["pos"], w, b["counts"], b["offsets"], b["gy"], b["gw"], stream=stream)
+        plan.norm(grads, b["res"], max_norm=1.0, stream=stream)
+    comp.set_param("variant", variant)
+    try:
+        want, got = buffers(), buffers()
+        run(want)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(got)
+        for rep in range(4):
+            for t in got.values():
+                t.zero_()
+            junk = [torch.full((1 << 18,), 7, device="cuda", dtype=torch.int32) for _ in range(4)]
+            run(buffers())
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(want[n], got[n]) for n in want), rep
+        for side in (torch.cuda.Stream(), torch.cuda.Stream().cuda_stream):
+            got = buffers()
+            torch.cuda.synchronize()
+            for _ in range(3):
+                run(got, stream=side)
+                junk = [torch.full((1 << 18,), 7, device="cuda", dtype=torch.int32) for _ in range(8)]
+            torch.cuda.synchronize()
+            assert all(torch.equal(want[n], got[n]) for n in want)
+    finally:
+        comp.set_param("variant", 0)
