@@ -18,16 +18,21 @@
          and 1 GiB per buffer
   copy   ccl_comp_copy at 64 MiB, 512 MiB and 3 GiB, and the bf16 <-> fp32 array converters at 2^28 elements
 
-    python bench_configs.py [--out results/configs.json] [--skip c3,batch,types,align,write,copy] [--only c1,c4] [--c3-k 7]
+  optimizer  what follows C4's reduce, from the reduced fusion buffer of its 256 tensors: the norm of all gradients, the AdamW
+         step with an fp32 copy of the weights and its states in 32 and in 8 bits
+  tokens 16,384 tokens x 8 of 128 experts, rows of 4,096 bf16: sort, dispatch, combine and both gradients; and 8 tokens
+
+    python bench_configs.py [--out results/configs.json] [--skip c3,batch,types,align,write,copy,optimizer,tokens] [--only c1,c4] [--c3-k 7]
                             [--set realign=0]
 
---only runs just the named sections (c1, c2, c3, batch, types, align, write, copy, c4, latency), --c3-k just the named sizes of
+--only runs just the named sections (c1, c2, c3, batch, types, align, write, copy, c4, optimizer, tokens, latency), --c3-k just the named sizes of
 the sweep (size = 1 KiB x 4^k): what a profiler run of one kernel wants.
 
 EVERY row is checked before it is timed: the first buffer set goes through the call once and the result is compared,
 bit for bit, with the CPU oracle (oracle/, the checker -- it is never the thing measured) on the same inputs: whole
-buffers up to 64 MiB, beyond that the first 16 MiB and the last 1 MiB of every buffer.  A row that fails the check ends
-the run.  Writes a JSON file and prints a markdown table.  Bytes are algorithmic: (N + 1) x chunk for a reduce,
+buffers up to 64 MiB, beyond that the first 16 MiB and the last 1 MiB of every buffer; the optimizer and token rows, which
+have no counterpart in the reference, with the same formula in 64 bits (2-norm of the difference under the type's half
+step).  A row that fails the check ends the run.  Writes a JSON file and prints a markdown table.  Bytes are algorithmic: (N + 1) x chunk for a reduce,
 2 x payload for pack and unpack.  Buffers of 64 MiB rotate over several sets so that the 256 MB Infinity Cache cannot
 hold them.
 """
@@ -451,6 +456,82 @@ def main():
             f"{us_three / us_fused:.2f}x faster than the 3-step sequence; {fused_kernel}")
         plan.close()
 
+    def verify_near(what, got, want, bound):
+        """2-norm of the difference over that of the result, at most `bound`."""
+        off = float((got.double() - want.double()).norm() / want.double().norm())
+        if not off <= bound:
+            sys.exit(f"CHECK FAILED: {what}: {off:.3g} off the result in 64 bits, {bound:.3g} allowed")
+        checked[0] += 1
+
+    # ---- the optimizer step on C4's tensors
+    if want("optimizer"):
+        rng = np.random.default_rng(4)
+        counts = [int(round(math.exp(rng.uniform(math.log(2048), math.log(2_097_152))))) for _ in range(256)]
+        plan = comp.FusionPlan(counts, comp.BFLOAT16, 512)      # 512 bytes: every tensor on a block of the 8-bit states
+        n, total = plan.elements, sum(counts)
+        inside = torch.zeros(n, dtype=torch.bool, device="cuda")
+        for i, c in enumerate(counts):
+            inside[plan.offset(i) // 2:plan.offset(i) // 2 + c] = True
+        grads = [(torch.randn(n, device="cuda") * 1e-3 * inside).bfloat16() for _ in range(3)]
+        master = torch.randn(n, device="cuda") * 0.02 * inside
+        flat = master.bfloat16()
+        params = [flat[plan.offset(i) // 2:plan.offset(i) // 2 + c] for i, c in enumerate(counts)]
+        result, ws = torch.zeros(2, device="cuda"), torch.empty(plan.norm_workspace, dtype=torch.uint8, device="cuda")
+        plan.norm(grads[0], result, multiplier=1 / 8, max_norm=1.0, workspace=ws)
+        norm = grads[0].double().norm() / 8
+        verify_near("gradient norm", result, torch.stack([norm, (1 / (norm + 1e-6)).clamp(max=1.0) / 8]), 18 * 2.0 ** -24)
+        us = timed(torch, lambda i: plan.norm(grads[i % 3], result, multiplier=1 / 8, max_norm=1.0, workspace=ws), 50, 10)
+        add("gradient norm and clip coefficient, 256 tensors in one fusion buffer", us, 2 * total)
+        hyper = dict(lr=3e-4, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, step=1, master=master, grad_scale=result[1:])
+        for eight in (False, True):
+            m, v = (torch.zeros(n, dtype=torch.uint8 if eight else torch.float32, device="cuda") for _ in range(2))
+            sc = torch.zeros(2 * -(-n // comp.STATE_BLOCK), dtype=torch.uint8, device="cuda") if eight else None
+            before, g = master.double(), grads[0].double() * result[1].double()
+            plan.adamw(params, grads[0], m, v, scales=sc, seed=1 if eight else None, **hyper)
+            verify_near("AdamW step", master, before * (1 - 3e-5) - 3e-4 * g / (g.abs() + 1e-8), 2.0 ** -24)
+            us = timed(torch, lambda i: plan.adamw(params, grads[i % 3], m, v, scales=sc, seed=1 if eight else None, **hyper), 50, 10)
+            add(f"AdamW step, 256 bf16 tensors with an fp32 copy, states in {'8 bits, stochastic' if eight else '32 bits'}", us,
+                total * (12 + (4 if eight else 16)) + (total // 64 if eight else 0))
+        plan.close()
+        del grads, master, flat, params, m, v, before, g
+
+    # ---- tokens to experts and back
+    for tokens in ((16384, 8) if want("tokens") else ()):
+        k, experts, hidden = 8, 128, 4096
+        ids = torch.randn(tokens, experts, device="cuda").topk(k, dim=1).indices.int()
+        pos = torch.zeros(tokens, k, dtype=torch.int32, device="cuda")
+        cnt, off = torch.zeros(experts, dtype=torch.int32, device="cuda"), torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+        nrows, row = tokens * k, 2 * hidden
+        x, y, out, gy, back, g = ([torch.randn(r, hidden, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
+                                 for r in (tokens, nrows, nrows, nrows, tokens, tokens))
+        w, gw = torch.softmax(torch.randn(tokens, k, device="cuda"), 1), torch.zeros(tokens, k, device="cuda")
+        comp.token_sort(ids, experts, pos, cnt, off)
+        order = torch.argsort(ids.reshape(-1), stable=True)
+        if not torch.equal(pos.reshape(-1)[order], torch.arange(nrows, device="cuda", dtype=torch.int32)):
+            sys.exit("CHECK FAILED: token sort")
+        checked[0] += 1
+        add(f"tokens: sort {tokens:,} x {k} by expert", timed(torch, lambda i: comp.token_sort(ids, experts, pos, cnt, off), 50, 10), 8 * nrows)
+        comp.token_dispatch(x[0], pos, cnt, off, out[0])
+        if not torch.equal(out[0], x[0][order // k]):
+            sys.exit("CHECK FAILED: token dispatch")
+        checked[0] += 1
+        add(f"tokens: dispatch {tokens:,} x {k} rows of 8 KiB", timed(torch, lambda i: comp.token_dispatch(x[i % 3], pos, cnt, off, out[i % 3]), 50, 10),
+            (tokens + nrows) * row)
+        comp.token_combine(y[0], pos, w, back[0])
+        taken = [y[0][pos[:, j].long()].double() for j in range(k)]
+        verify_near("token combine", back[0], sum(w[:, j, None].double() * taken[j] for j in range(k)), 2.0 ** -8)
+        add(f"tokens: combine {tokens:,} x {k} rows", timed(torch, lambda i: comp.token_combine(y[i % 3], pos, w, back[i % 3]), 50, 10), (tokens + nrows) * row)
+        comp.token_combine_backward(g[0], y[0], pos, w, cnt, off, gy[0], gw)
+        verify_near("combine's gradient, weights", gw, torch.stack([(taken[j] * g[0].double()).sum(1) for j in range(k)], 1), 2.0 ** -18)
+        verify_near("combine's gradient, rows", gy[0], w.reshape(-1)[order, None].double() * g[0][order // k].double(), 2.0 ** -8)
+        add(f"tokens: combine's gradient, {tokens:,} x {k} rows", timed(torch, lambda i: comp.token_combine_backward(g[i % 3], y[i % 3], pos, w, cnt, off, gy[i % 3], gw), 50, 10),
+            (tokens + 2 * nrows) * row)
+        comp.token_dispatch_backward(y[0], pos, back[0])
+        verify_near("dispatch's gradient", back[0], sum(taken), 2.0 ** -8)
+        add(f"tokens: dispatch's gradient, {tokens:,} x {k} rows", timed(torch, lambda i: comp.token_dispatch_backward(y[i % 3], pos, back[i % 3]), 50, 10),
+            (tokens + nrows) * row)
+        del x, y, out, gy, back, g, taken
+
     # small-message latency from C++ (no Python in the loop); the program checks its own results
     lat = os.path.join(ROOT, "tests", "cpp", "bench_latency")
     lat_lines = []
@@ -466,7 +547,8 @@ def main():
     os.makedirs(os.path.dirname(args.out), exist_ok=True)
     with open(args.out, "w") as f:
         json.dump(res, f, indent=1)
-    print(f"Every row below was checked bit for bit against the CPU oracle before it was timed ({checked[0]} checks).\n")
+    print(f"Every row below was checked before it was timed, bit for bit against the CPU oracle or (optimizer, tokens) against 64 bits "
+          f"({checked[0]} checks).\n")
     print("| configuration | algorithmic bytes | us per call | GB/s | of 8 TB/s | note |")
     print("|---|---|---|---|---|---|")
     print("\n".join(rows))
