@@ -232,7 +232,7 @@ def _check_tensors(what, tensors, dtype, least, here):
         raise ValueError(f"{what}: not contiguous")
     if kinds != {dtype}:
         raise ValueError(f"{what}: {kinds}, {dtype} is wanted")
-    if any(map(operator.lt, sizes, least)):
+    if sizes != least and any(map(operator.lt, sizes, least)):
         raise ValueError(f"{what}: a tensor has fewer elements than the plan says")
 
 

@@ -149,10 +149,11 @@ void backward_by_dot(const BackwardArgs& a) {
 
 // ---- rows in the order of the buffer
 
-// Where it pays: from 64 MiB of rows, as far as HIP takes the blocks in one launch.  16,384 tokens x 8 rows of 8 KiB, dispatch
-// and combine's gradient: 184 and 377 us against 239 and 440 token by token; x 4 of 14 KiB, 8,192 tokens: 91 and 172
-// against 127 and 202; one row of 8 KiB each, 65,536 tokens: 184 and 267 against 186 and 301.  At 33 MiB (2,048 x 2 of 8 KiB) the
-// launch in front costs as much as it gains: 13 and 20 us against 11 and 19.  "variant" 8 takes it at any size.
+// Where it pays: from 64 MiB of rows, as far as HIP takes the blocks in one launch.  Against token by token, with buffers that
+// the 256 MB cache cannot hold: dispatch of 16,384 tokens x 8 rows of 8 KiB 217 against 247 us, both gradients of 8,192 x 8 291
+// against 318; dispatch and combine's gradient of 8,192 x 4 rows of 14 KiB 91 and 172 against 127 and 202, of 65,536 x 1 of 8 KiB
+// 184 and 267 against 186 and 301.  At 33 MiB (2,048 x 2 of 8 KiB) the launch in front costs what it gains: 13 and 20 us
+// against 11 and 19.  "variant" 8 takes it at any size.
 constexpr uint64_t kOrderBytes = 64u << 20;
 bool wants_order(int dtype, size_t n_tokens, int top_k, size_t hidden) {
     const uint64_t entries = (uint64_t)n_tokens * (uint64_t)top_k;
