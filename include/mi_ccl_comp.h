@@ -262,7 +262,9 @@ typedef struct mi_ccl_adamw_options {
     const int64_t* step_ptr;    /* device, or NULL: read in place of `step` (a step captured into a graph) */
     const float* lr_ptr;        /* device, or NULL: read in place of `lr` */
     const float* grad_scale;    /* device, or NULL for 1: every gradient is multiplied with it; not finite = no step */
+    void* workspace;            /* with step_ptr or lr_ptr: MI_CCL_ADAMW_WORKSPACE bytes on the device, needed by this call alone */
 } mi_ccl_adamw_options;
+#define MI_CCL_ADAMW_WORKSPACE 16
 
 /* One AdamW step (decoupled weight decay) over all tensors of the plan: with g = grad_scale * gradient,
  *   exp_avg    = beta1 * exp_avg + (1 - beta1) * g

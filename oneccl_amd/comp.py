@@ -44,13 +44,14 @@ EXPORTS = [
 
 STATE_FP32, STATE_8BIT = 0, 1          # formats of the AdamW states
 STATE_BLOCK = 256                      # elements that share a scale in the 8-bit format
+ADAMW_WORKSPACE = 16                   # bytes, of a step whose number or learning rate is read from the device
 
 
 class AdamwOptions(C.Structure):
     """mi_ccl_adamw_options"""
     _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
                 ("step", C.c_int64), ("seed", C.c_uint64), ("stochastic", C.c_int), ("step_ptr", C.c_void_p), ("lr_ptr", C.c_void_p),
-                ("grad_scale", C.c_void_p)]
+                ("grad_scale", C.c_void_p), ("workspace", C.c_void_p)]
 
 
 class CclError(RuntimeError):
@@ -433,10 +434,11 @@ class FusionPlan:
         _check(lib().mi_ccl_fusion_norm(self._h, lst, buf, multiplier, max_norm, res, ws, size, _stream(stream)), "mi_ccl_fusion_norm")
 
     def adamw(self, params, grads, exp_avg, exp_avg_sq, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, step=1, scales=None,
-              master=None, grad_scale=None, seed=None, step_ptr=None, lr_ptr=None, stream=None):
+              master=None, grad_scale=None, seed=None, step_ptr=None, lr_ptr=None, workspace=None, stream=None):
         """One AdamW step over the plan's tensors, in place.  States: float32 (32 bits) or uint8 (8 bits, with `scales`) in the
         plan's layout.  seed: not None rounds 8-bit states stochastically.  step_ptr (int64), lr_ptr and grad_scale (float32):
-        one-element device tensors read by the kernel."""
+        one-element device tensors read by the kernel.  workspace: with step_ptr or lr_ptr, ADAMW_WORKSPACE bytes; allocated for
+        the call when None."""
         import torch
         here = self._device()
         if len(params) != self.k or params[0] is None:
@@ -446,9 +448,12 @@ class FusionPlan:
         kind = torch.uint8 if eight else torch.float32
         m, v = _memory("exp_avg", exp_avg, kind, self.elements, here), _memory("exp_avg_sq", exp_avg_sq, kind, self.elements, here)
         sc = _memory("scales", scales, torch.uint8, 2 * ((self.elements + STATE_BLOCK - 1) // STATE_BLOCK), here) if eight else None
+        ws, size, _keep = _workspace(workspace, ADAMW_WORKSPACE if step_ptr is not None or lr_ptr is not None else 0, here, stream)
+        if workspace is not None and size < ADAMW_WORKSPACE:
+            raise ValueError(f"workspace: {size} bytes, {ADAMW_WORKSPACE} are needed")
         o = AdamwOptions(lr, beta1, beta2, eps, weight_decay, int(step), 0 if seed is None else int(seed), int(seed is not None),
                          _optional("step_ptr", step_ptr, torch.int64, 1, here), _optional("lr_ptr", lr_ptr, torch.float32, 1, here),
-                         _optional("grad_scale", grad_scale, torch.float32, 1, here))
+                         _optional("grad_scale", grad_scale, torch.float32, 1, here), ws)
         lst, buf = self._gradients(grads, here)
         _check(lib().mi_ccl_fusion_adamw(self._h, _kind(params[0]), _tensor_array(params), lst, buf, STATE_8BIT if eight else STATE_FP32,
                                          m, v, sc, _optional("master", master, torch.float32, self.elements, here), C.byref(o),

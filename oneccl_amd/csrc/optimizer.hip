@@ -14,6 +14,11 @@ bool float_type(int dtype) {
     return dtype == MI_CCL_FLOAT32 || dtype == MI_CCL_FLOAT16 || dtype == MI_CCL_BFLOAT16;
 }
 
+// A device address that the kernels' 48-bit tables hold, at a multiple of the element size.
+bool address_ok(const void* p, size_t esz) {
+    return p && (uintptr_t)p % esz == 0 && ((uint64_t)(uintptr_t)p >> 48) == 0;
+}
+
 // the gradients of a call: every tensor of its own, or one fusion buffer in the plan's layout
 bool gradients_ok(const mi_ccl_fusion_plan* plan, const void* const* grads, const void* fusion_buf) {
     if ((grads != nullptr) == (fusion_buf != nullptr))
@@ -21,15 +26,13 @@ bool gradients_ok(const mi_ccl_fusion_plan* plan, const void* const* grads, cons
     if (fusion_buf)
         return (uintptr_t)fusion_buf % plan->esz == 0;
     for (size_t t = 0; t < plan->k; t++)
-        if (plan->counts[t] && (!grads[t] || (uintptr_t)grads[t] % plan->esz))
+        if (plan->counts[t] && !address_ok(grads[t], plan->esz))
             return false;
     return true;
 }
 
-bool set_pointers(FusionPtrs& to, const void* const* from, size_t t0, size_t t1) {
-    for (size_t t = t0; t < t1; t++)
-        if (!to.set(t - t0, from[t])) return false;
-    return true;
+void set_pointers(FusionPtrs& to, const void* const* from, size_t t0, size_t t1) {
+    for (size_t t = t0; t < t1; t++) to.set(t - t0, from[t]);      // the address of an empty tensor may be anything: it is not used
 }
 
 // ---- norm
@@ -160,8 +163,8 @@ int mi_ccl_fusion_norm(mi_ccl_fusion_plan* plan, const void* const* grads, const
         const uint32_t blocks = norm_blocks(plan, t0, t1);
         if (blocks == 0)
             continue;
-        if (!fusion_buf && !set_pointers(ptrs, grads, t0, t1))
-            return MI_CCL_INVALID_ARGUMENTS;
+        if (!fusion_buf)
+            set_pointers(ptrs, grads, t0, t1);
         NormTables tb = { plan->d_off, plan->d_bytes, plan->d_items + plan->item_begin[t0],
                           (uint32_t)(plan->item_begin[t1] - plan->item_begin[t0]), (uint32_t)t0 };
         g_last_kernel = "fusion_norm_kernel";
@@ -189,6 +192,8 @@ int mi_ccl_fusion_adamw(mi_ccl_fusion_plan* plan, int param_dtype, void* const* 
         return MI_CCL_INVALID_ARGUMENTS;
     if ((uintptr_t)o->step_ptr % sizeof(int64_t) || (uintptr_t)o->lr_ptr % sizeof(float) || (uintptr_t)o->grad_scale % sizeof(float))
         return MI_CCL_INVALID_ARGUMENTS;
+    if ((o->step_ptr || o->lr_ptr) && (!o->workspace || (uintptr_t)o->workspace % alignof(AdamwDerived)))
+        return MI_CCL_INVALID_ARGUMENTS;
     if (master && param_dtype == MI_CCL_FLOAT32)
         return MI_CCL_INVALID_ARGUMENTS;
     if (eight && (!blocks_aligned(plan) || (plan->total_bytes && !scales)))
@@ -199,7 +204,7 @@ int mi_ccl_fusion_adamw(mi_ccl_fusion_plan* plan, int param_dtype, void* const* 
         return MI_CCL_INVALID_ARGUMENTS;
     const size_t psize = fusion_dtype_size(param_dtype);
     for (size_t t = 0; t < plan->k; t++)
-        if (plan->counts[t] && (!params[t] || (uintptr_t)params[t] % psize))
+        if (plan->counts[t] && !address_ok(params[t], psize))
             return MI_CCL_INVALID_ARGUMENTS;
 
     FusionPtrs pp = {}, gg = {};
@@ -216,24 +221,28 @@ int mi_ccl_fusion_adamw(mi_ccl_fusion_plan* plan, int param_dtype, void* const* 
     sc.beta2 = (float)o->beta2;
     sc.rest2 = (float)(1.0 - o->beta2);
     sc.eps = (float)o->eps;
-    sc.lr_ptr = o->lr_ptr;
-    sc.step_ptr = o->step_ptr;
     sc.grad_scale = o->grad_scale;
-    sc.lr = o->lr;
-    sc.weight_decay = o->weight_decay;
-    sc.beta1_d = o->beta1;
-    sc.beta2_d = o->beta2;
-    sc.step = o->step_ptr ? 1 : o->step;
-    sc.seed = o->seed;
-    adamw_derive(sc);
+    const AdamwHyper h = { o->lr, o->weight_decay, o->beta1, o->beta2, o->step_ptr ? 1 : o->step, o->seed };
+    sc.d = adamw_derive(h);
+    sc.derived = nullptr;
+    if ((o->step_ptr || o->lr_ptr) && plan->item_begin[plan->k]) {
+        AdamwDerived* derived = (AdamwDerived*)o->workspace;
+        g_last_kernel = "adamw_derive_kernel";
+        hipLaunchKernelGGL(adamw_derive_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, h, o->lr_ptr, o->step_ptr, derived);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess)
+            return fusion_status_of(e);
+        sc.derived = derived;
+    }
 
     const int state = !eight ? STATE_FP32 : o->stochastic ? STATE_RANDOM : STATE_NEAREST;
     const uint32_t subs = kFusionChunk / (uint32_t)plan->esz / kAdamwTile;
     const uint64_t most = items_per_launch(subs);
     for (size_t t0 = 0; t0 < plan->k; t0 += kFusionGroup) {
         const size_t t1 = (t0 + kFusionGroup < plan->k) ? t0 + kFusionGroup : plan->k;
-        if (!set_pointers(pp, (const void* const*)params, t0, t1) || (!fusion_buf && grads && !set_pointers(gg, grads, t0, t1)))
-            return MI_CCL_INVALID_ARGUMENTS;
+        set_pointers(pp, (const void* const*)params, t0, t1);
+        if (!fusion_buf && grads)
+            set_pointers(gg, grads, t0, t1);
         a.tb.t0 = (uint32_t)t0;
         for (uint64_t i0 = plan->item_begin[t0]; i0 < plan->item_begin[t1]; i0 += most) {
             const uint64_t i1 = (i0 + most < plan->item_begin[t1]) ? i0 + most : plan->item_begin[t1];

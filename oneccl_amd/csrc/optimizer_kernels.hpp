@@ -321,19 +321,24 @@ __device__ __forceinline__ void store_codes(uint8_t* p, Span n, uint32_t c) {
 
 // ---- AdamW --------------------------------------------------------------------------------------------------------------
 
-struct AdamwScalars {
-    float beta1, rest1, beta2, rest2, eps;
+// What follows from the learning rate and the step's number.
+struct AdamwDerived {
     float decay;            // 1 - lr wd
     float step_size;        // lr / (1 - beta1^t)
     float root_scale;       // 1 / sqrt(1 - beta2^t)
     uint32_t key;           // of the step's random bits
-    // on the device, where the host does not know them: the learning rate, the step, the factor of the gradients
-    const float* lr_ptr;
-    const int64_t* step_ptr;
-    const float* grad_scale;
-    double lr, weight_decay, beta1_d, beta2_d;
+};
+static_assert(sizeof(AdamwDerived) == MI_CCL_ADAMW_WORKSPACE, "the header says how much memory it takes");
+struct AdamwHyper {
+    double lr, weight_decay, beta1, beta2;
     int64_t step;
     uint64_t seed;
+};
+struct AdamwScalars {
+    float beta1, rest1, beta2, rest2, eps;
+    AdamwDerived d;
+    const AdamwDerived* derived;    // or NULL: in memory, from numbers that the host does not know
+    const float* grad_scale;
 };
 
 // b^t by squaring, in fp64
@@ -345,11 +350,20 @@ __host__ __device__ inline double whole_power(double b, int64_t t) {
     }
     return r;
 }
-__host__ __device__ inline void adamw_derive(AdamwScalars& a) {
-    a.decay = (float)(1.0 - a.lr * a.weight_decay);
-    a.step_size = (float)(a.lr / (1.0 - whole_power(a.beta1_d, a.step)));
-    a.root_scale = (float)(1.0 / sqrt(1.0 - whole_power(a.beta2_d, a.step)));
-    a.key = step_key(a.seed, (uint64_t)a.step);
+__host__ __device__ inline AdamwDerived adamw_derive(const AdamwHyper& h) {
+    AdamwDerived d;
+    d.decay = (float)(1.0 - h.lr * h.weight_decay);
+    d.step_size = (float)(h.lr / (1.0 - whole_power(h.beta1, h.step)));
+    d.root_scale = (float)(1.0 / sqrt(1.0 - whole_power(h.beta2, h.step)));
+    d.key = step_key(h.seed, (uint64_t)h.step);
+    return d;
+}
+// A launch of its own: the some 200 fp64 instructions in every wave of the step would make it a third slower (130 M parameters with
+// 8-bit states 471 against 337 us).
+__global__ void adamw_derive_kernel(AdamwHyper h, const float* lr, const int64_t* step, AdamwDerived* out) {
+    if (lr) h.lr = (double)*lr;
+    if (step) h.step = *step;
+    *out = adamw_derive(h);
 }
 
 struct AdamwTables {
@@ -376,8 +390,8 @@ __device__ __forceinline__ float scaled_sqrt(float v, float scale) {
 __device__ __forceinline__ void adamw_element(const AdamwScalars& a, float g, float& m, float& v, float& x) {
     m = m * a.beta1 + g * a.rest1;
     v = v * a.beta2 + (g * g) * a.rest2;
-    const float root = scaled_sqrt(v, a.root_scale) + a.eps;
-    x = x * a.decay - (m * __builtin_amdgcn_rcpf(root)) * a.step_size;
+    const float root = scaled_sqrt(v, a.d.root_scale) + a.eps;
+    x = x * a.d.decay - (m * __builtin_amdgcn_rcpf(root)) * a.d.step_size;
 }
 
 // A tensor's arrays, each at the tensor's element 0.
@@ -445,7 +459,7 @@ __device__ __forceinline__ void adamw_tile(const AdamwTensor& t, int64_t e0, con
             for (int i = 0; i < 4; i++)
                 if (!n.has(i)) m[i] = v[i] = 0.0f;              // no part of the block
         }
-        const Coded c = encode4<STATE == STATE_RANDOM>(m, v, t.at + e0 + e, a.key);
+        const Coded c = encode4<STATE == STATE_RANDOM>(m, v, t.at + e0 + e, a.d.key);
         store_codes<WHOLE>(avg8 + e, n, c.cm);
         store_codes<WHOLE>(sq8 + e, n, c.cv);
         if ((WHOLE || n.to) && (threadIdx.x & 63u) == 0) {
@@ -473,11 +487,7 @@ fusion_adamw_kernel(FusionPtrs params, FusionPtrs grads, const unsigned char* bu
         scale = *a.grad_scale;
         if (!(fabsf(scale) < __builtin_inff())) return;         // gradients that are not finite: no step
     }
-    if (a.lr_ptr || a.step_ptr) {
-        if (a.lr_ptr) a.lr = (double)*a.lr_ptr;
-        if (a.step_ptr) a.step = *a.step_ptr;
-        adamw_derive(a);
-    }
+    if (a.derived) a.d = *a.derived;
     const FusionItem w = tb.items[blockIdx.x / kSubs];
     const uint64_t tile = (uint64_t)w.c * kSubs + blockIdx.x % kSubs, off = tb.off[w.t];
     AdamwTensor t;

@@ -415,6 +415,8 @@ def test_refusals(comp):
         with pytest.raises(refused):
             c.step(**dict(HYPER, **kw))
     with pytest.raises(refused):
+        c.step(lr_ptr=torch.zeros(1, device="cuda"), workspace=torch.zeros(8, dtype=torch.uint8, device="cuda"), **HYPER)
+    with pytest.raises(refused):
         c.step(**dict(HYPER, seed=1))                                    # 32-bit states have nothing to round
     for kw in (dict(grad_scale=torch.zeros(1, device="cuda", dtype=torch.float64)), dict(step_ptr=torch.zeros(1, device="cuda")),
                dict(lr_ptr=torch.zeros(1))):
@@ -445,6 +447,9 @@ def test_refusals(comp):
     import ctypes as C
     P = comp._ptr_array(c.params)
     args = [c.plan._h, comp.BFLOAT16, P, None, c.buffer.data_ptr(), 0, c.m.data_ptr(), c.v.data_ptr(), None, None, C.byref(o), None]
+    o.lr_ptr = c.m.data_ptr()                                            # and nowhere to put what follows from it
+    assert L.mi_ccl_fusion_adamw(*args) == comp.INVALID_ARGUMENTS
+    o.lr_ptr = None
     for i, x in ((1, comp.INT8), (2, None), (3, P), (4, None), (4, c.buffer.data_ptr() + 1), (5, 2), (6, None), (7, c.v.data_ptr() + 2), (9, c.m.data_ptr() + 1), (10, None)):
         bad = list(args)
         bad[i] = x
