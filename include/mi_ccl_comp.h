@@ -303,7 +303,7 @@ int mi_ccl_token_rows(size_t n_tokens, int top_k, int n_experts, size_t align, s
 
 /* expert_ids: n_tokens x top_k ids, row after row, INT32 or INT64 (index_dtype).  Writes positions[n_tokens x top_k], the row of each
  * entry in the sorted buffer or -1; counts[n_experts], the entries that each expert keeps; offsets[n_experts + 1], the first
- * row of each expert and the end of the last.  workspace: mi_ccl_token_sort_workspace bytes (0 for up to 8,192 entries),
+ * row of each expert and the end of the last.  workspace: mi_ccl_token_sort_workspace bytes (0 for up to 4,096 entries),
  * needed by this call alone.  With n_tokens == 0 counts and offsets become zero. */
 int mi_ccl_token_sort_workspace(size_t n_tokens, int top_k, int n_experts, size_t* bytes);
 int mi_ccl_token_sort(int index_dtype, const void* expert_ids, size_t n_tokens, int top_k, int n_experts, size_t align,

@@ -74,7 +74,7 @@ int launched(const char* name) {
 template <class I>
 int sort_launch(const I* ids, uint32_t n, uint32_t experts, uint32_t align, uint32_t capacity, int32_t* positions, int32_t* counts,
                 int32_t* offsets, uint32_t* table, hipStream_t stream) {
-    const SortShape s = sort_shape(n);
+    const SortShape s = sort_shape(n, experts);
     if (s.runs > 1) {
         hipLaunchKernelGGL((token_count_kernel<I>), dim3(s.runs), dim3(kSortBlock), 0, stream, ids, n, experts, s.run, table);
         const int rc = launched("token_count_kernel");
@@ -227,7 +227,7 @@ int mi_ccl_token_sort_workspace(size_t n_tokens, int top_k, int n_experts, size_
     uint64_t entries = 0, r = 0;
     if (!bytes || !token_sizes(n_tokens, top_k, n_experts, 1, 0, &entries, &r))
         return MI_CCL_INVALID_ARGUMENTS;
-    const SortShape s = sort_shape((uint32_t)entries);
+    const SortShape s = sort_shape((uint32_t)entries, (uint32_t)n_experts);
     *bytes = s.runs > 1 ? (size_t)s.runs * (size_t)n_experts * sizeof(uint32_t) : 0;
     return MI_CCL_SUCCESS;
 }

@@ -18,21 +18,25 @@ namespace mi {
 // A stable counting sort.  A block of 16 waves takes a contiguous run of entries, a wave a sixteenth of it.  Up to
 // kSortSingle entries one block does everything in one launch; beyond, a first launch counts the experts of every run
 // (runs x E numbers in the workspace) and in a second every block adds up the runs before its own, which costs each block
-// a read of that table (at most 512 rows out of L2) and saves the launch of a scan between the two.
+// a read of that table and saves the launch of a scan between the two.  What bounds it is latency: the passes of a block over its
+// run, and the table, which grows with the number of runs; the two meet at about 2 sqrt(n / E) runs.  Measured as nodes of a
+// replayed graph: 2,048 entries 4.9 us, 4,096 6.9, 8,192 7.3 (in one block 11), 131,072 over 128 experts 9.8 (64 runs; 10.9 with 128,
+// 11.2 with 32), 524,288 over 256 19.2 (128 runs; 20.2 with 64, 25.3 with 256), 2,097,152 over 128 25 (256 runs; 50 with 64).
 constexpr int kSortBlock = 1024;
 constexpr int kSortWaves = kSortBlock / 64;
 constexpr int kSortMaxExperts = 1024;
-constexpr uint32_t kSortSingle = 8192;      // entries one block sorts alone
+constexpr uint32_t kSortSingle = 4096;      // entries one block sorts alone
 constexpr uint32_t kSortRun = 2048;         // fewest entries of a block's run
-constexpr uint32_t kSortMaxRuns = 512;
 
 // runs and entries per run of a sort of n entries (a run is a whole number of entries per lane)
 struct SortShape {
     uint32_t runs, run;
 };
-inline SortShape sort_shape(uint32_t n) {
+inline SortShape sort_shape(uint32_t n, uint32_t experts) {
     if (n <= kSortSingle) return SortShape{ 1, ((n + kSortBlock - 1) / kSortBlock) * kSortBlock };
-    uint32_t run = (uint32_t)(((uint64_t)n + kSortMaxRuns - 1) / kSortMaxRuns);
+    uint32_t runs = 16;
+    while (runs < 512 && (uint64_t)runs * runs * experts < 4ull * n) runs++;
+    uint32_t run = (uint32_t)(((uint64_t)n + runs - 1) / runs);
     run = (run + kSortBlock - 1) / kSortBlock * kSortBlock;
     if (run < kSortRun) run = kSortRun;
     return SortShape{ (uint32_t)(((uint64_t)n + run - 1) / run), run };

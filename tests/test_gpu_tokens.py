@@ -61,7 +61,7 @@ def sort(comp, ids, experts, align=1, capacity=0, kind="int32"):
 @pytest.mark.parametrize("tokens,k,experts,align,capacity,kind", [
     (1, 1, 1, 1, 0, "int32"), (1, 8, 64, 1, 0, "int64"), (3, 2, 5, 4, 0, "int32"), (64, 1, 3, 1, 7, "int32"), (65, 1, 1, 1, 0, "int64"),
     (1000, 3, 17, 16, 0, "int32"), (1024, 8, 256, 1, 0, "int32"), (8192, 1, 257, 8, 5, "int32"), (8193, 1, 1024, 1, 0, "int64"),
-    (2049, 4, 128, 128, 0, "int32"), (20000, 6, 60, 1, 1999, "int32"), (7, 300, 2, 1, 0, "int32"), (300001, 8, 1000, 1, 0, "int32"), (0, 4, 9, 8, 0, "int32"),
+    (2049, 4, 128, 128, 0, "int32"), (20000, 6, 60, 1, 1999, "int32"), (7, 300, 2, 1, 0, "int32"), (4096, 1, 7, 1, 0, "int32"), (4097, 1, 7, 4, 0, "int64"), (300001, 8, 1000, 1, 0, "int32"), (0, 4, 9, 8, 0, "int32"),
 ])
 def test_sort(comp, tokens, k, experts, align, capacity, kind):
     rng = np.random.default_rng(tokens + experts)

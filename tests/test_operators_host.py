@@ -19,8 +19,8 @@ def test_rows_and_workspace():
     assert c.token_rows(1, 2, 8, align=16) == 2 + 2 * 15          # no more experts than entries have rows to pad
     assert c.token_rows(1000, 2, 8, capacity=10) == 80
     assert c.token_rows(1000, 2, 8, align=4, capacity=10) == 80 + 8 * 3
-    assert c.token_sort_workspace(4096, 2, 64) == 0
-    assert c.token_sort_workspace(4097, 2, 64) > 0
+    assert c.token_sort_workspace(2048, 2, 64) == 0
+    assert c.token_sort_workspace(2049, 2, 64) > 0
     for args in ((1, 0, 1, 1, 0), (1, 1, 0, 1, 0), (1, 1, 1025, 1, 0), (1, 1, 1, 0, 0), (1 << 31, 1, 1, 1, 0), (1 << 30, 2, 1, 1, 0),
                  (1 << 22, 1, 1024, 1 << 22, 0), (1, 1, 1, 1 << 31, 0), (1, 1, 1, 1, 1 << 31)):
         with pytest.raises(c.CclError):
