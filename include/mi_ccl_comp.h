@@ -231,7 +231,7 @@ int mi_ccl_fusion_reduce_static(const size_t* counts, size_t k, int dtype, size_
 /* result[0] = |multiplier| * sqrt(sum of the squares of all gradients), result[1] = the factor that a clipped step
  * multiplies its gradients with: multiplier * min(1, max_norm / (result[0] + 1e-6)), or multiplier when max_norm <= 0.
  * multiplier: what the gradients are yet to be multiplied with (1 / peers after a sum, 1 / loss scale).  A norm that is not
- * finite (squares are fp32: an element from 1.8e19 up overflows) gives result[1] = NaN, which mi_ccl_fusion_adamw takes as
+ * finite (squares are fp32: an element from 1.8e19 up overflows, one below 1e-19 counts for less than it is) gives result[1] = NaN, which mi_ccl_fusion_adamw takes as
  * "no step".  result: two floats on the device.  workspace: mi_ccl_fusion_norm_workspace bytes of device memory, 8-byte
  * aligned, needed by this call alone (calls that may overlap take one each).  The sum has a fixed order: the same
  * gradients give the same bits. */
@@ -273,7 +273,8 @@ typedef struct mi_ccl_adamw_options {
  * in fp32; 8-bit states are rounded after the weights have taken the exact ones.  params: HOST array of k device pointers
  * of param_dtype (FLOAT32, FLOAT16, BFLOAT16).  master: NULL, or for 16-bit weights the fp32 copy (in the plan's layout)
  * that is stepped in their place; the weights are then its rounding (to nearest even).  A grad_scale that is not finite
- * leaves weights and states as they are.  Tensors that are parameters twice must be one tensor of the plan.  Parameter
+ * leaves weights and states as they are.  lr and weight_decay >= 0, beta1 and beta2 in [0, 1), eps >= 2^-126 (the smallest
+ * normal float: it is what divides the update of a weight that never had a gradient).  Tensors that are parameters twice must be one tensor of the plan.  Parameter
  * groups with hyperparameters of their own take plans of their own. */
 int mi_ccl_fusion_adamw(mi_ccl_fusion_plan* plan, int param_dtype, void* const* params, const void* const* grads,
                         const void* fusion_buf, int state_format, void* exp_avg, void* exp_avg_sq, void* scales, float* master,

@@ -551,6 +551,14 @@ def token_order_workspace(dtype, n_tokens, top_k, hidden):
     return r.value
 
 
+def _weights(what, t, positions, here):
+    """Address of fp32 numbers, one per entry; None for None."""
+    import torch
+    if t is not None and t.shape != positions.shape:
+        _refuse(what, t, f"{tuple(positions.shape)}, the shape of positions,")
+    return _optional(what, t, torch.float32, 0, here)
+
+
 def _positions(positions, tokens, here):
     import torch
     shape = positions.shape
@@ -583,7 +591,7 @@ def token_combine(y, positions, weights, out, stream=None):
     rows, ldy, py = _rows("y", y, hidden, y.dtype, here)
     n, ldo, po = _rows("out", out, hidden, y.dtype, here)
     k, pos = _positions(positions, n, here)
-    _check(lib().mi_ccl_token_combine(_kind(y), py, ldy, rows, pos, _optional("weights", weights, torch.float32, n * k, here), n, k, hidden, po, ldo,
+    _check(lib().mi_ccl_token_combine(_kind(y), py, ldy, rows, pos, _weights("weights", weights, positions, here), n, k, hidden, po, ldo,
                                       _stream(stream)), "mi_ccl_token_combine")
 
 
@@ -607,10 +615,10 @@ def token_combine_backward(grad_out, y, positions, weights, counts, offsets, gra
     dtype = _kind(grad_out)
     ws, size, _keep = _workspace(workspace, token_order_workspace(dtype, n, k, hidden), here, stream)
     _check(lib().mi_ccl_token_combine_backward(dtype, pg, ldg, py, ldy, rows, pos,
-                                               _optional("weights", weights, torch.float32, n * k, here),
+                                               _weights("weights", weights, positions, here),
                                                _memory("counts", counts, torch.int32, experts, here),
                                                _memory("offsets", offsets, torch.int32, experts + 1, here), experts, n, k, hidden, pd, ldd,
-                                               _optional("grad_weights", grad_weights, torch.float32, n * k, here), ws, size, _stream(stream)),
+                                               _weights("grad_weights", grad_weights, positions, here), ws, size, _stream(stream)),
            "mi_ccl_token_combine_backward")
 
 

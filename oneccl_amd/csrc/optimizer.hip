@@ -187,7 +187,7 @@ int mi_ccl_fusion_adamw(mi_ccl_fusion_plan* plan, int param_dtype, void* const* 
     if (!eight && state_format != MI_CCL_STATE_FP32)
         return MI_CCL_INVALID_ARGUMENTS;
     // what makes no sense is refused; the comparisons are false for NaN
-    if (!(o->lr >= 0.0) || !(o->beta1 >= 0.0 && o->beta1 < 1.0) || !(o->beta2 >= 0.0 && o->beta2 < 1.0) || !(o->eps >= 0.0) ||
+    if (!(o->lr >= 0.0) || !(o->beta1 >= 0.0 && o->beta1 < 1.0) || !(o->beta2 >= 0.0 && o->beta2 < 1.0) || !(o->eps >= 0x1p-126) ||
         !(o->weight_decay >= 0.0) || (!o->step_ptr && o->step < 1) || (o->stochastic != 0 && (o->stochastic != 1 || !eight)))
         return MI_CCL_INVALID_ARGUMENTS;
     if ((uintptr_t)o->step_ptr % sizeof(int64_t) || (uintptr_t)o->lr_ptr % sizeof(float) || (uintptr_t)o->grad_scale % sizeof(float))

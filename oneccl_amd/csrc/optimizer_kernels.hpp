@@ -125,8 +125,7 @@ fusion_norm_finish_kernel(const double* partial, uint32_t n, double multiplier, 
 // ---- 8-bit states -------------------------------------------------------------------------------------------------------
 
 // The largest of a number over the wave (which holds one block), the same in every lane: within rows of 16 lanes with
-// DPP, whose exchange is part of the max instruction, across the four rows on the scalar unit.  (Through the LDS crossbar, a
-// shuffle per step, this was a tenth of the 8-bit step's instructions.)
+// DPP, whose exchange is part of the max instruction, across the four rows on the scalar unit: no trip through the LDS crossbar.
 template <int CTRL>
 __device__ __forceinline__ uint32_t max_across(uint32_t x) {
     const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);

@@ -221,6 +221,27 @@ def test_a_gradient_that_is_not_finite_reaches_its_own_element_alone(comp, eight
     assert np.array_equal(w[~mask], w2[~mask])
 
 
+@pytest.mark.parametrize("grad", ["float32", "bfloat16"])
+def test_the_smallest_gradients_and_eps(comp, grad):
+    """Second moments that are denormal (gradients from 1e-22 to 1e-17) with an eps that they matter beside, and weights without
+    any gradient: nothing becomes infinite or NaN, and the update is the formula's (m and v of a first step are exact multiples;
+    their denormal values are off by half of 2^-149, which the root of v feels as sqrt(2^-149) at most)."""
+    import torch
+    n = 3000
+    plan = comp.FusionPlan([n], code(comp, grad), 1)
+    g = torch.zeros(n, dtype=getattr(torch, grad), device="cuda")
+    g[1000:] = torch.logspace(-22, -17, 2000, device="cuda").to(g.dtype)
+    p, m, v = (torch.zeros(plan.elements, device="cuda") for _ in range(3))
+    eps = 1e-20
+    plan.adamw([p], [g], m, v, lr=1.0, beta1=0.9, beta2=0.95, eps=eps, weight_decay=0.0, step=1)
+    assert not p[:1000].any() and torch.isfinite(p).all()
+    x = g[1000:].double().cpu().numpy()
+    want = -x / (x + eps)
+    root_off = math.sqrt(2.0 ** -149 / 0.05)                            # sqrt(v + 2^-149) - sqrt(v) is at most sqrt(2^-149)
+    tol = 20 * U + root_off / (x + eps) + 2.0 ** -149 / 0.1 / (x + eps)
+    assert (np.abs(p[1000:].double().cpu().numpy() - want) <= tol).all()
+
+
 def test_a_fresh_state_and_zero_gradients(comp):
     """All-zero 8-bit states; a zero gradient moves a weight by its decay alone, states stay zero."""
     import torch
@@ -411,7 +432,7 @@ def test_refusals(comp):
     c = Case(comp, [300, 5], "bfloat16", "bfloat16", True)
     e = Case(comp, [300, 5], "bfloat16", "bfloat16", True, eight=True)
     refused = (ValueError, comp.CclError)
-    for kw in (dict(lr=-1.0), dict(lr=math.nan), dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0), dict(weight_decay=-1.0), dict(step=0)):
+    for kw in (dict(lr=-1.0), dict(lr=math.nan), dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0), dict(eps=0.0), dict(eps=1e-40), dict(weight_decay=-1.0), dict(step=0)):
         with pytest.raises(refused):
             c.step(**dict(HYPER, **kw))
     with pytest.raises(refused):

@@ -333,6 +333,8 @@ def test_refusals_of_the_binding(comp):
                  lambda: comp.token_dispatch(x, pos.long(), counts, offsets, torch.zeros(4, 8, device="cuda")),
                  lambda: comp.token_combine(x.t(), pos, None, torch.zeros(2, 2, device="cuda")),
                  lambda: comp.token_combine(x.double(), pos, None, torch.zeros(2, 8, device="cuda").double()),
+                 lambda: comp.token_combine(x, pos, torch.zeros(2, 3, device="cuda"), torch.zeros(2, 8, device="cuda")),
+                 lambda: comp.token_combine(x, pos, torch.zeros(2, 2, device="cuda").t(), torch.zeros(2, 8, device="cuda").double()),
                  lambda: comp.token_combine(x, pos, torch.zeros(3, device="cuda"), torch.zeros(2, 8, device="cuda")),
                  lambda: comp.token_combine_backward(x, None, pos, None, counts, offsets, torch.zeros(4, 8, device="cuda"), torch.zeros(2, 2, device="cuda")),
                  lambda: comp.token_combine_backward(x, torch.zeros(3, 8, device="cuda"), pos, None, counts, offsets, torch.zeros(4, 8, device="cuda")),
