@@ -161,10 +161,14 @@ bool wants_order(int dtype, size_t n_tokens, int top_k, size_t hidden) {
         return false;
     return entries * hidden * fusion_dtype_size(dtype) >= kOrderBytes || mi_ccl_get_param("variant") == 8;
 }
-uint32_t order_lanes(uint32_t nvec) {
-    uint32_t lanes = 64;
-    while (lanes < nvec && lanes < 512) lanes <<= 1;
-    return lanes;
+// Lanes of an entry, 64 to 512.  Dispatch takes no fewer than the row has vectors (one load and one store each); the gradient,
+// which has more to do per vector, lets a third of them go round twice.  26,296 tokens x 5 rows of 139 vectors: dispatch 76 us with 256
+// lanes, 83 with 128; gradient 158 with 128, 206 with 256.  65,536 x 1 rows of 230 vectors: gradient 132 with 256, 143 with 128.
+// Under 256 lanes a block of 256 takes several entries (26,296 x 8 rows of 64 vectors: dispatch 40 us, 51 in blocks of 64).
+uint32_t order_log_lanes(uint32_t nvec, bool one_each) {
+    uint32_t log_lanes = 6;
+    while (log_lanes < 9 && (one_each ? (1u << log_lanes) : (3u << log_lanes) / 2) < nvec) log_lanes++;
+    return log_lanes;
 }
 // Entries per run: what keeps the run's tokens within 2 MiB, half of an XCD's L2, and leaves every XCD a run.  Measured at 8
 // choices and 8 KiB: 16,384 tokens 184 us with 2,048 entries, 190 with 1,024, 193 with 512, 201 with 256; at 4 choices and 14 KiB,
@@ -174,9 +178,12 @@ uint32_t order_log_run(uint64_t entries, uint32_t top_k, uint64_t row_bytes) {
     while (log_run < 11 && ((2ull << log_run) / top_k) * row_bytes <= (2u << 20) && (16ull << log_run) <= entries) log_run++;
     return log_run;
 }
-uint32_t order_blocks(uint64_t entries, uint32_t log_run) {         // eight runs at a time
+uint32_t order_block(uint32_t log_lanes) {
+    return log_lanes < 8 ? 256u : 1u << log_lanes;
+}
+uint32_t order_blocks(uint64_t entries, uint32_t log_run, uint32_t log_lanes) {         // eight runs at a time
     const uint64_t runs = (entries + (1u << log_run) - 1) >> log_run;
-    return (uint32_t)(((runs + 7) / 8 * 8) << log_run);
+    return (uint32_t)((((runs + 7) / 8 * 8) << log_run) / (order_block(log_lanes) >> log_lanes));
 }
 uint32_t order_pad_blocks(int n_experts) {      // a multiple of the XCDs, which the blocks behind count on
     return ((uint32_t)n_experts * kPadParts + 7) / 8 * 8;
@@ -189,14 +196,42 @@ int order_launch(const int32_t* positions, uint64_t entries, uint32_t log_run, s
     return launched("token_order_kernel");
 }
 
+struct OrderedArgs {
+    dim3 grid, block;
+    hipStream_t stream;
+    uint32_t pads, log_lanes, log_run;
+    uint64_t entries;
+    const OrderedEntry* order;
+    bool multi() const { return log_lanes < 8; }
+};
+template <class E, bool MULTI>
+void dispatch_ordered_launch(const OrderedArgs& o, const RowShape& s, const void* x, size_t ld_x, const int32_t* counts, const int32_t* offsets,
+                             void* out, size_t ld_out, size_t rows) {
+    hipLaunchKernelGGL((token_dispatch_ordered_kernel<E, MULTI>), o.grid, o.block, 0, o.stream, (const unsigned char*)x, (uint64_t)ld_x, s.nvec, s.tail,
+                       s.top_k, o.entries, o.pads, o.order, o.log_lanes, o.log_run, counts, offsets, (unsigned char*)out, (uint64_t)ld_out,
+                       (uint64_t)rows);
+}
+template <class E>
+void dispatch_ordered(const OrderedArgs& o, const RowShape& s, const void* x, size_t ld_x, const int32_t* counts, const int32_t* offsets, void* out,
+                      size_t ld_out, size_t rows) {
+    if (o.multi()) dispatch_ordered_launch<E, true>(o, s, x, ld_x, counts, offsets, out, ld_out, rows);
+    else dispatch_ordered_launch<E, false>(o, s, x, ld_x, counts, offsets, out, ld_out, rows);
+}
+
+template <class V, bool DOT, bool MULTI>
+void backward_ordered_launch(const OrderedArgs& o, const BackwardArgs& a) {
+    hipLaunchKernelGGL((token_backward_ordered_kernel<V, DOT, MULTI>), o.grid, o.block, 0, o.stream, (const unsigned char*)a.grad, (uint64_t)a.ld_grad,
+                       (const unsigned char*)a.y, (uint64_t)a.ld_y, a.s.nvec, a.s.tail, a.s.top_k, o.entries, o.pads, o.order, o.log_lanes, o.log_run,
+                       a.weights, a.counts, a.offsets, (unsigned char*)a.grad_y, (uint64_t)a.ld_grad_y, (uint64_t)a.rows, a.grad_weights);
+}
 template <class V, bool DOT>
 void backward_ordered(const BackwardArgs& a, const OrderedEntry* order, uint32_t log_run) {
     const uint64_t entries = a.s.tokens * a.s.top_k;
-    const uint32_t pads = order_pad_blocks(a.n_experts);
-    hipLaunchKernelGGL((token_backward_ordered_kernel<V, DOT>), dim3(pads + order_blocks(entries, log_run)), dim3(order_lanes(a.s.nvec)), 0, a.stream,
-                       (const unsigned char*)a.grad, (uint64_t)a.ld_grad, (const unsigned char*)a.y, (uint64_t)a.ld_y, a.s.nvec, a.s.tail, a.s.top_k,
-                       entries, pads, order, log_run, a.weights, a.counts, a.offsets, (unsigned char*)a.grad_y, (uint64_t)a.ld_grad_y, (uint64_t)a.rows,
-                       a.grad_weights);
+    const uint32_t pads = order_pad_blocks(a.n_experts), log_lanes = order_log_lanes(a.s.nvec, false);
+    const OrderedArgs o = { dim3(pads + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), a.stream, pads, log_lanes, log_run,
+                            entries, order };
+    if (o.multi()) backward_ordered_launch<V, DOT, true>(o, a);
+    else backward_ordered_launch<V, DOT, false>(o, a);
 }
 template <class V>
 void backward_ordered_by_dot(const BackwardArgs& a, const OrderedEntry* order, uint32_t log_run) {
@@ -274,16 +309,11 @@ int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens
         const int rc = order_launch(positions, entries, log_run, out_rows, order, (hipStream_t)stream);
         if (rc != MI_CCL_SUCCESS)
             return rc;
-        const uint32_t pads = order_pad_blocks(n_experts);
-        const dim3 grid(pads + order_blocks(entries, log_run)), block(order_lanes(s.nvec));
-        if (fusion_dtype_size(dtype) == 4)
-            hipLaunchKernelGGL((token_dispatch_ordered_kernel<uint32_t>), grid, block, 0, (hipStream_t)stream, (const unsigned char*)x, (uint64_t)ld_x,
-                               s.nvec, s.tail, s.top_k, entries, pads, (const OrderedEntry*)order, log_run, counts, offsets, (unsigned char*)out,
-                               (uint64_t)ld_out, (uint64_t)out_rows);
-        else
-            hipLaunchKernelGGL((token_dispatch_ordered_kernel<uint16_t>), grid, block, 0, (hipStream_t)stream, (const unsigned char*)x, (uint64_t)ld_x,
-                               s.nvec, s.tail, s.top_k, entries, pads, (const OrderedEntry*)order, log_run, counts, offsets, (unsigned char*)out,
-                               (uint64_t)ld_out, (uint64_t)out_rows);
+        const uint32_t pads = order_pad_blocks(n_experts), log_lanes = order_log_lanes(s.nvec, true);
+        const OrderedArgs o = { dim3(pads + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), (hipStream_t)stream, pads, log_lanes,
+                                log_run, entries, order };
+        if (fusion_dtype_size(dtype) == 4) dispatch_ordered<uint32_t>(o, s, x, ld_x, counts, offsets, out, ld_out, out_rows);
+        else dispatch_ordered<uint16_t>(o, s, x, ld_x, counts, offsets, out, ld_out, out_rows);
         return launched("token_dispatch_ordered_kernel");
     }
     const uint32_t pad_blocks = (uint32_t)n_experts * kPadParts;

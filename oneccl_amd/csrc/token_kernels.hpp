@@ -267,88 +267,99 @@ token_order_kernel(const int32_t* positions, uint64_t n, uint32_t run, uint64_t 
     }
 }
 
-// The entry of a block: run after run, eight runs side by side, one per XCD (blocks go round the XCDs by their index).
-__device__ __forceinline__ uint64_t ordered_index(uint32_t block, uint32_t log_run) {
-    const uint32_t xcd = block & 7u, r = block >> 3;
-    return ((((uint64_t)(r >> log_run) << 3) + xcd) << log_run) + (r & ((1u << log_run) - 1));
-}
+// A block takes one entry, or, MULTI, an entry per group of 1 << log_lanes lanes: whole waves, so that all that follows from the
+// entry is on the scalar unit (as the lanes' own values it cost a tenth).  Entries come run after run, eight runs side by
+// side, one per XCD (blocks go round the XCDs by their index).
+constexpr int kOrderedBlock = 512;         // lanes at most
+template <bool MULTI>
+struct OrderedLane {
+    uint64_t at;                // the group's place in the order
+    uint32_t lanes, lane;
+    __device__ __forceinline__ OrderedLane(uint32_t block, uint32_t log_lanes, uint32_t log_run) {
+        lanes = MULTI ? 1u << log_lanes : blockDim.x;
+        lane = MULTI ? threadIdx.x & (lanes - 1) : threadIdx.x;
+        const uint32_t xcd = block & 7u;
+        const uint32_t r = MULTI ? (block >> 3) * (blockDim.x >> log_lanes) + __builtin_amdgcn_readfirstlane(threadIdx.x >> log_lanes) : block >> 3;
+        at = ((((uint64_t)(r >> log_run) << 3) + xcd) << log_run) + (r & ((1u << log_run) - 1));
+    }
+};
 
-// A block copies one entry's row.
-template <class E>
-__global__ void __launch_bounds__(512)
+// A group of lanes copies one entry's row.
+template <class E, bool MULTI>
+__global__ void __launch_bounds__(kOrderedBlock)
 token_dispatch_ordered_kernel(const unsigned char* x, uint64_t ldx, uint32_t nvec, uint32_t tail, uint32_t top_k, uint64_t n, uint32_t pad_blocks,
-                              const OrderedEntry* order, uint32_t log_run, const int32_t* counts, const int32_t* offsets, unsigned char* out, uint64_t ldo,
-                              uint64_t rows) {
+                              const OrderedEntry* order, uint32_t log_lanes, uint32_t log_run, const int32_t* counts, const int32_t* offsets,
+                              unsigned char* out, uint64_t ldo, uint64_t rows) {
     constexpr uint32_t VEC = 16 / sizeof(E);
     if (blockIdx.x < pad_blocks) {
         clear_padding<E>(blockIdx.x, counts, offsets, rows, out, ldo, nvec, tail);
         return;
     }
-    const uint64_t at = ordered_index(blockIdx.x - pad_blocks, log_run);
-    if (at >= n) return;
-    const OrderedEntry e = order[at];
+    const OrderedLane<MULTI> my(blockIdx.x - pad_blocks, log_lanes, log_run);
+    if (my.at >= n) return;
+    const OrderedEntry e = order[my.at];
     if (e.row < 0) return;
+    const uint32_t lane = my.lane;
     const unsigned char* src = x + (uint64_t)(e.entry / top_k) * ldx * sizeof(E);
     unsigned char* o = out + (uint64_t)e.row * ldo * sizeof(E);
-    for (uint32_t v = threadIdx.x; v < nvec; v += blockDim.x) st_loose((u32x4_u*)o + v, ((const u32x4_u*)src)[v]);
-    if (threadIdx.x < tail) st_elem<E>(o, (uint64_t)nvec * VEC + threadIdx.x, ld_elem<E>(src, (uint64_t)nvec * VEC + threadIdx.x));
+    for (uint32_t v = lane; v < nvec; v += my.lanes) st_loose((u32x4_u*)o + v, ((const u32x4_u*)src)[v]);
+    if (lane < tail) st_elem<E>(o, (uint64_t)nvec * VEC + lane, ld_elem<E>(src, (uint64_t)nvec * VEC + lane));
 }
 
-// A block takes one entry: its row's gradient and, with DOT, its weight's.  The dot product is summed lane by lane over the
-// columns, then over the wave and the block in a fixed order.
-template <class V, bool DOT>
-__global__ void __launch_bounds__(512)
+// A group of lanes takes one entry: its row's gradient and, with DOT, its weight's.  The dot product is summed lane by lane over
+// the columns, then over the wave and the group's waves in a fixed order.
+template <class V, bool DOT, bool MULTI>
+__global__ void __launch_bounds__(kOrderedBlock)
 token_backward_ordered_kernel(const unsigned char* grad, uint64_t ldg, const unsigned char* y, uint64_t ldy, uint32_t nvec, uint32_t tail,
-                              uint32_t top_k, uint64_t n, uint32_t pad_blocks, const OrderedEntry* order, uint32_t log_run, const float* weights,
-                              const int32_t* counts, const int32_t* offsets, unsigned char* grad_y, uint64_t ldd, uint64_t rows,
-                              float* grad_weights) {
+                              uint32_t top_k, uint64_t n, uint32_t pad_blocks, const OrderedEntry* order, uint32_t log_lanes, uint32_t log_run,
+                              const float* weights, const int32_t* counts, const int32_t* offsets, unsigned char* grad_y, uint64_t ldd,
+                              uint64_t rows, float* grad_weights) {
     typedef typename V::elem_t E;
     constexpr int VEC = V::VEC;
     if (blockIdx.x < pad_blocks) {
         clear_padding<E>(blockIdx.x, counts, offsets, rows, grad_y, ldd, nvec, tail);
         return;
     }
-    const uint64_t at = ordered_index(blockIdx.x - pad_blocks, log_run);
-    if (at >= n) return;
-    const OrderedEntry e = order[at];
-    if (e.row < 0) {
-        if (DOT && threadIdx.x == 0) grad_weights[e.entry] = 0.0f;
-        return;
-    }
-    __shared__ float part[8];
-    const float f = weights ? weights[e.entry] : 1.0f;
-    const unsigned char* g = grad + (uint64_t)(e.entry / top_k) * ldg * sizeof(E);
-    const unsigned char* r = DOT ? y + (uint64_t)e.row * ldy * sizeof(E) : nullptr;
-    unsigned char* d = grad_y + (uint64_t)e.row * ldd * sizeof(E);
+    __shared__ float part[kOrderedBlock / 64];
+    const OrderedLane<MULTI> my(blockIdx.x - pad_blocks, log_lanes, log_run);
+    const uint32_t lane = my.lane;
+    OrderedEntry e = { -1, 0 };
+    if (my.at < n) e = order[my.at];
     float dot = 0.0f;
-    for (uint32_t v = threadIdx.x; v < nvec; v += blockDim.x) {
-        u32x4 b;
-        if (DOT) b = ld_loose((const u32x4_u*)r + v);
-        float a[VEC], c[VEC];
-        V::widen(((const u32x4_u*)g)[v], a);
+    if (e.row >= 0) {
+        const float f = weights ? weights[e.entry] : 1.0f;
+        const unsigned char* g = grad + (uint64_t)(e.entry / top_k) * ldg * sizeof(E);
+        const unsigned char* r = DOT ? y + (uint64_t)e.row * ldy * sizeof(E) : nullptr;
+        unsigned char* d = grad_y + (uint64_t)e.row * ldd * sizeof(E);
+        for (uint32_t v = lane; v < nvec; v += my.lanes) {
+            u32x4 b;
+            if (DOT) b = ld_loose((const u32x4_u*)r + v);
+            float a[VEC], c[VEC];
+            V::widen(((const u32x4_u*)g)[v], a);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) c[i] = f * a[i];
-        st_loose((u32x4_u*)d + v, V::narrow(c));
-        if (DOT) {
-            V::widen(b, c);
+            for (int i = 0; i < VEC; i++) c[i] = f * a[i];
+            st_loose((u32x4_u*)d + v, V::narrow(c));
+            if (DOT) {
+                V::widen(b, c);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) dot = __builtin_fmaf(a[i], c[i], dot);
+                for (int i = 0; i < VEC; i++) dot = __builtin_fmaf(a[i], c[i], dot);
+            }
         }
-    }
-    if (threadIdx.x < tail) {
-        const uint64_t i = (uint64_t)nvec * VEC + threadIdx.x;
-        const float a = V::widen1(ld_elem<E>(g, i));
-        st_elem<E>(d, i, V::narrow1(f * a));
-        if (DOT) dot = __builtin_fmaf(a, V::widen1(ld_elem<E>(r, i)), dot);
+        if (lane < tail) {
+            const uint64_t i = (uint64_t)nvec * VEC + lane;
+            const float a = V::widen1(ld_elem<E>(g, i));
+            st_elem<E>(d, i, V::narrow1(f * a));
+            if (DOT) dot = __builtin_fmaf(a, V::widen1(ld_elem<E>(r, i)), dot);
+        }
     }
     if (DOT) {
         dot = wave_sum(dot);
         if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = dot;
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (lane == 0 && my.at < n) {
             float sum = 0.0f;
-            for (uint32_t q = 0; q < blockDim.x / 64; q++) sum += part[q];
-            grad_weights[e.entry] = sum;
+            for (uint32_t q = 0; q < my.lanes / 64; q++) sum += part[(threadIdx.x >> 6) + q];
+            grad_weights[e.entry] = sum;            // 0 for an entry without a row
         }
     }
 }
