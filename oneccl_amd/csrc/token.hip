@@ -170,12 +170,17 @@ uint32_t order_log_lanes(uint32_t nvec, bool one_each) {
     while (log_lanes < 9 && (one_each ? (1u << log_lanes) : (3u << log_lanes) / 2) < nvec) log_lanes++;
     return log_lanes;
 }
-// Entries per run: what keeps the run's tokens within 2 MiB, half of an XCD's L2, and leaves every XCD a run.  Measured at 8
-// choices and 8 KiB: 16,384 tokens 184 us with 2,048 entries, 190 with 1,024, 193 with 512, 201 with 256; at 4 choices and 14 KiB,
-// 8,192 tokens: 116, 93, 91, 90.
+// Entries per run: what keeps the run's tokens within 2 MiB, half of an XCD's L2, and leaves no XCD without a run in a tenth of the
+// turns (an XCD takes every eighth run).  Dispatch, two buffer sets in turn: 16,384 tokens x 8 of 8 KiB 184 us with 2,048 entries, 190 with
+// 1,024, 193 with 512, 201 with 256; 8,192 x 4 of 14 KiB 116, 93, 91, 90; 5,000 x 8 of 8 KiB, 20 runs of 2,048 or 40 of 1,024, 67 and 60;
+// 2,304 x 8, 9 runs of 2,048 or 36 of 512, 42 and 30.
 uint32_t order_log_run(uint64_t entries, uint32_t top_k, uint64_t row_bytes) {
     uint32_t log_run = 8;
-    while (log_run < 11 && ((2ull << log_run) / top_k) * row_bytes <= (2u << 20) && (16ull << log_run) <= entries) log_run++;
+    while (log_run < 11 && ((2ull << log_run) / top_k) * row_bytes <= (2u << 20)) log_run++;
+    for (; log_run > 8; log_run--) {
+        const uint64_t runs = (entries + (1u << log_run) - 1) >> log_run, turns = (runs + 7) / 8;
+        if (10 * runs >= 9 * 8 * turns) break;
+    }
     return log_run;
 }
 uint32_t order_block(uint32_t log_lanes) {
