@@ -95,10 +95,10 @@ constexpr int kDispatchU = 1;
 constexpr int kCombineU = 2;
 
 template <class E>
-void dispatch_launch(const RowShape& s, dim3 grid, uint32_t pad_blocks, hipStream_t stream, const void* x, size_t ld_x, const int32_t* positions,
+void dispatch_launch(const RowShape& s, uint32_t experts, hipStream_t stream, const void* x, size_t ld_x, const int32_t* positions,
                      const int32_t* counts, const int32_t* offsets, void* out, size_t ld_out, size_t rows) {
-    hipLaunchKernelGGL((token_dispatch_kernel<E, kDispatchU>), grid, dim3(kBlock), 0, stream, (const unsigned char*)x, (uint64_t)ld_x, s,
-                       pad_blocks, positions, counts, offsets, (unsigned char*)out, (uint64_t)ld_out, (uint64_t)rows);
+    hipLaunchKernelGGL((token_dispatch_kernel<E, kDispatchU>), dim3(column_blocks(s), pad_blocks(experts) + token_blocks(s)), dim3(kBlock), 0, stream,
+                       (const unsigned char*)x, (uint64_t)ld_x, s, experts, positions, counts, offsets, (unsigned char*)out, (uint64_t)ld_out, (uint64_t)rows);
 }
 
 template <class V, int K>
@@ -118,8 +118,7 @@ void combine_by_k(const RowShape& s, hipStream_t stream, const void* y, size_t l
 
 struct BackwardArgs {
     RowShape s;
-    uint32_t block, pad_blocks, grid;
-    int n_experts;
+    uint32_t block, grid, experts;
     hipStream_t stream;
     const void *grad, *y;
     size_t ld_grad, ld_y, ld_grad_y, rows;
@@ -131,7 +130,7 @@ struct BackwardArgs {
 template <class V, int K, bool DOT>
 void backward_launch(const BackwardArgs& a) {
     hipLaunchKernelGGL((token_combine_backward_kernel<V, K, DOT>), dim3(a.grid), dim3(a.block), 0, a.stream, (const unsigned char*)a.grad,
-                       (uint64_t)a.ld_grad, (const unsigned char*)a.y, (uint64_t)a.ld_y, (uint64_t)a.rows, a.s, a.pad_blocks, a.positions,
+                       (uint64_t)a.ld_grad, (const unsigned char*)a.y, (uint64_t)a.ld_y, (uint64_t)a.rows, a.s, a.experts, a.positions,
                        a.weights, a.counts, a.offsets, (unsigned char*)a.grad_y, (uint64_t)a.ld_grad_y, a.grad_weights);
 }
 template <class V, bool DOT>
@@ -190,9 +189,6 @@ uint32_t order_blocks(uint64_t entries, uint32_t log_run, uint32_t log_lanes) { 
     const uint64_t runs = (entries + (1u << log_run) - 1) >> log_run;
     return (uint32_t)((((runs + 7) / 8 * 8) << log_run) / (order_block(log_lanes) >> log_lanes));
 }
-uint32_t order_pad_blocks(int n_experts) {      // a multiple of the XCDs, which the blocks behind count on
-    return ((uint32_t)n_experts * kPadParts + 7) / 8 * 8;
-}
 int order_launch(const int32_t* positions, uint64_t entries, uint32_t log_run, size_t rows, OrderedEntry* order, hipStream_t stream) {
     uint32_t shift = 0;
     while (((uint64_t)(rows - 1) >> shift) >= kOrderBuckets) shift++;
@@ -204,7 +200,7 @@ int order_launch(const int32_t* positions, uint64_t entries, uint32_t log_run, s
 struct OrderedArgs {
     dim3 grid, block;
     hipStream_t stream;
-    uint32_t pads, log_lanes, log_run;
+    uint32_t experts, log_lanes, log_run;
     uint64_t entries;
     const OrderedEntry* order;
     bool multi() const { return log_lanes < 8; }
@@ -213,7 +209,7 @@ template <class E, bool MULTI>
 void dispatch_ordered_launch(const OrderedArgs& o, const RowShape& s, const void* x, size_t ld_x, const int32_t* counts, const int32_t* offsets,
                              void* out, size_t ld_out, size_t rows) {
     hipLaunchKernelGGL((token_dispatch_ordered_kernel<E, MULTI>), o.grid, o.block, 0, o.stream, (const unsigned char*)x, (uint64_t)ld_x, s.nvec, s.tail,
-                       s.top_k, o.entries, o.pads, o.order, o.log_lanes, o.log_run, counts, offsets, (unsigned char*)out, (uint64_t)ld_out,
+                       s.top_k, o.entries, o.experts, o.order, o.log_lanes, o.log_run, counts, offsets, (unsigned char*)out, (uint64_t)ld_out,
                        (uint64_t)rows);
 }
 template <class E>
@@ -226,15 +222,15 @@ void dispatch_ordered(const OrderedArgs& o, const RowShape& s, const void* x, si
 template <class V, bool DOT, bool MULTI>
 void backward_ordered_launch(const OrderedArgs& o, const BackwardArgs& a) {
     hipLaunchKernelGGL((token_backward_ordered_kernel<V, DOT, MULTI>), o.grid, o.block, 0, o.stream, (const unsigned char*)a.grad, (uint64_t)a.ld_grad,
-                       (const unsigned char*)a.y, (uint64_t)a.ld_y, a.s.nvec, a.s.tail, a.s.top_k, o.entries, o.pads, o.order, o.log_lanes, o.log_run,
+                       (const unsigned char*)a.y, (uint64_t)a.ld_y, a.s.nvec, a.s.tail, a.s.top_k, o.entries, o.experts, o.order, o.log_lanes, o.log_run,
                        a.weights, a.counts, a.offsets, (unsigned char*)a.grad_y, (uint64_t)a.ld_grad_y, (uint64_t)a.rows, a.grad_weights);
 }
 template <class V, bool DOT>
 void backward_ordered(const BackwardArgs& a, const OrderedEntry* order, uint32_t log_run) {
     const uint64_t entries = a.s.tokens * a.s.top_k;
-    const uint32_t pads = order_pad_blocks(a.n_experts), log_lanes = order_log_lanes(a.s.nvec, false);
-    const OrderedArgs o = { dim3(pads + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), a.stream, pads, log_lanes, log_run,
-                            entries, order };
+    const uint32_t log_lanes = order_log_lanes(a.s.nvec, false);
+    const OrderedArgs o = { dim3(pad_blocks(a.experts) + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), a.stream, a.experts,
+                            log_lanes, log_run, entries, order };
     if (o.multi()) backward_ordered_launch<V, DOT, true>(o, a);
     else backward_ordered_launch<V, DOT, false>(o, a);
 }
@@ -314,19 +310,17 @@ int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens
         const int rc = order_launch(positions, entries, log_run, out_rows, order, (hipStream_t)stream);
         if (rc != MI_CCL_SUCCESS)
             return rc;
-        const uint32_t pads = order_pad_blocks(n_experts), log_lanes = order_log_lanes(s.nvec, true);
-        const OrderedArgs o = { dim3(pads + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), (hipStream_t)stream, pads, log_lanes,
-                                log_run, entries, order };
+        const uint32_t experts = (uint32_t)n_experts, log_lanes = order_log_lanes(s.nvec, true);
+        const OrderedArgs o = { dim3(pad_blocks(experts) + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), (hipStream_t)stream,
+                                experts, log_lanes, log_run, entries, order };
         if (fusion_dtype_size(dtype) == 4) dispatch_ordered<uint32_t>(o, s, x, ld_x, counts, offsets, out, ld_out, out_rows);
         else dispatch_ordered<uint16_t>(o, s, x, ld_x, counts, offsets, out, ld_out, out_rows);
         return launched("token_dispatch_ordered_kernel");
     }
-    const uint32_t pad_blocks = (uint32_t)n_experts * kPadParts;
-    const dim3 grid(column_blocks(s), pad_blocks + token_blocks(s));
     if (fusion_dtype_size(dtype) == 4)
-        dispatch_launch<uint32_t>(s, grid, pad_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
+        dispatch_launch<uint32_t>(s, (uint32_t)n_experts, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
     else
-        dispatch_launch<uint16_t>(s, grid, pad_blocks, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
+        dispatch_launch<uint16_t>(s, (uint32_t)n_experts, (hipStream_t)stream, x, ld_x, positions, counts, offsets, out, ld_out, out_rows);
     return launched("token_dispatch_kernel");
 }
 
@@ -370,9 +364,8 @@ int mi_ccl_token_combine_backward(int dtype, const void* grad_out, size_t ld_gra
     const uint32_t most = n_tokens >= 256 ? 512 : 1024;
     a.block = 64;
     while (a.block < a.s.nvec && a.block < most) a.block <<= 1;
-    a.n_experts = n_experts;
-    a.pad_blocks = (uint32_t)n_experts * kPadParts;
-    a.grid = a.pad_blocks + (uint32_t)(n_tokens < (1u << 20) ? n_tokens : 1u << 20);
+    a.experts = (uint32_t)n_experts;
+    a.grid = pad_blocks(a.experts) + (uint32_t)(n_tokens < (1u << 20) ? n_tokens : 1u << 20);
     a.stream = (hipStream_t)stream;
     a.grad = grad_out;
     a.ld_grad = ld_grad;

@@ -182,14 +182,19 @@ struct RowShape {
     uint64_t tokens;
 };
 
-// Clears the rows of padding behind one expert's rows, every kPadParts-th of them; pad_blocks = experts * kPadParts blocks do
-// all.  They come first in the grid: behind the tokens' they would be what a launch waits for at its end.
+// Clears the rows of padding behind one expert's rows, every kPadParts-th of them; pad_blocks(experts) blocks do
+// all.  They come first in the grid: behind the tokens' they would be what a launch waits for at its end.  Their number is a
+// multiple of the XCDs, so that the block behind them has the first one; with an odd number of experts the last ones are idle.
 constexpr uint32_t kPadParts = 4;
+__host__ __device__ constexpr uint32_t pad_blocks(uint32_t experts) {
+    return (experts * kPadParts + 7) / 8 * 8;
+}
 template <class E>
-__device__ __forceinline__ void clear_padding(uint32_t block, const int32_t* counts, const int32_t* offsets, uint64_t rows,
+__device__ __forceinline__ void clear_padding(uint32_t block, uint32_t experts, const int32_t* counts, const int32_t* offsets, uint64_t rows,
                                               unsigned char* out, uint64_t ld, uint32_t nvec, uint32_t tail) {
     constexpr uint32_t VEC = 16 / sizeof(E);
     const uint32_t expert = block / kPadParts;
+    if (expert >= experts) return;
     const int64_t r0 = (int64_t)offsets[expert] + counts[expert];
     int64_t r1 = offsets[expert + 1];
     if (r0 < 0) return;
@@ -287,15 +292,16 @@ struct OrderedLane {
 // A group of lanes copies one entry's row.
 template <class E, bool MULTI>
 __global__ void __launch_bounds__(kOrderedBlock)
-token_dispatch_ordered_kernel(const unsigned char* x, uint64_t ldx, uint32_t nvec, uint32_t tail, uint32_t top_k, uint64_t n, uint32_t pad_blocks,
+token_dispatch_ordered_kernel(const unsigned char* x, uint64_t ldx, uint32_t nvec, uint32_t tail, uint32_t top_k, uint64_t n, uint32_t experts,
                               const OrderedEntry* order, uint32_t log_lanes, uint32_t log_run, const int32_t* counts, const int32_t* offsets,
                               unsigned char* out, uint64_t ldo, uint64_t rows) {
     constexpr uint32_t VEC = 16 / sizeof(E);
-    if (blockIdx.x < pad_blocks) {
-        clear_padding<E>(blockIdx.x, counts, offsets, rows, out, ldo, nvec, tail);
+    const uint32_t pads = pad_blocks(experts);
+    if (blockIdx.x < pads) {
+        clear_padding<E>(blockIdx.x, experts, counts, offsets, rows, out, ldo, nvec, tail);
         return;
     }
-    const OrderedLane<MULTI> my(blockIdx.x - pad_blocks, log_lanes, log_run);
+    const OrderedLane<MULTI> my(blockIdx.x - pads, log_lanes, log_run);
     if (my.at >= n) return;
     const OrderedEntry e = order[my.at];
     if (e.row < 0) return;
@@ -311,17 +317,18 @@ token_dispatch_ordered_kernel(const unsigned char* x, uint64_t ldx, uint32_t nve
 template <class V, bool DOT, bool MULTI>
 __global__ void __launch_bounds__(kOrderedBlock)
 token_backward_ordered_kernel(const unsigned char* grad, uint64_t ldg, const unsigned char* y, uint64_t ldy, uint32_t nvec, uint32_t tail,
-                              uint32_t top_k, uint64_t n, uint32_t pad_blocks, const OrderedEntry* order, uint32_t log_lanes, uint32_t log_run,
+                              uint32_t top_k, uint64_t n, uint32_t experts, const OrderedEntry* order, uint32_t log_lanes, uint32_t log_run,
                               const float* weights, const int32_t* counts, const int32_t* offsets, unsigned char* grad_y, uint64_t ldd,
                               uint64_t rows, float* grad_weights) {
     typedef typename V::elem_t E;
     constexpr int VEC = V::VEC;
-    if (blockIdx.x < pad_blocks) {
-        clear_padding<E>(blockIdx.x, counts, offsets, rows, grad_y, ldd, nvec, tail);
+    const uint32_t pads = pad_blocks(experts);
+    if (blockIdx.x < pads) {
+        clear_padding<E>(blockIdx.x, experts, counts, offsets, rows, grad_y, ldd, nvec, tail);
         return;
     }
     __shared__ float part[kOrderedBlock / 64];
-    const OrderedLane<MULTI> my(blockIdx.x - pad_blocks, log_lanes, log_run);
+    const OrderedLane<MULTI> my(blockIdx.x - pads, log_lanes, log_run);
     const uint32_t lane = my.lane;
     OrderedEntry e = { -1, 0 };
     if (my.at < n) e = order[my.at];
@@ -369,14 +376,15 @@ token_backward_ordered_kernel(const unsigned char* grad, uint64_t ldg, const uns
 // A token's columns are read once and stored to its rows.
 template <class E, int U>
 __global__ void __launch_bounds__(kBlock)
-token_dispatch_kernel(const unsigned char* x, uint64_t ldx, RowShape s, uint32_t pad_blocks, const int32_t* positions, const int32_t* counts,
+token_dispatch_kernel(const unsigned char* x, uint64_t ldx, RowShape s, uint32_t experts, const int32_t* positions, const int32_t* counts,
                       const int32_t* offsets, unsigned char* out, uint64_t ldo, uint64_t rows) {
     constexpr uint32_t VEC = 16 / sizeof(E);
-    if (blockIdx.y < pad_blocks) {
-        if (blockIdx.x == 0) clear_padding<E>(blockIdx.y, counts, offsets, rows, out, ldo, s.nvec, s.tail);
+    const uint32_t pads = pad_blocks(experts);
+    if (blockIdx.y < pads) {
+        if (blockIdx.x == 0) clear_padding<E>(blockIdx.y, experts, counts, offsets, rows, out, ldo, s.nvec, s.tail);
         return;
     }
-    const uint32_t token_block = blockIdx.y - pad_blocks, token_blocks = gridDim.y - pad_blocks;
+    const uint32_t token_block = blockIdx.y - pads, token_blocks = gridDim.y - pads;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t per_block = (kBlock / 64) >> s.log_waves, width = 64u << s.log_waves;
     const uint32_t col = (wave & ((1u << s.log_waves) - 1)) * 64u + lane;
@@ -464,17 +472,18 @@ token_combine_kernel(const unsigned char* y, uint64_t ldy, uint64_t rows, RowSha
 template <class V, int K, bool DOT>
 __global__ void __launch_bounds__(1024)
 token_combine_backward_kernel(const unsigned char* grad, uint64_t ldg, const unsigned char* y, uint64_t ldy, uint64_t rows, RowShape s,
-                              uint32_t pad_blocks, const int32_t* positions, const float* weights, const int32_t* counts,
+                              uint32_t experts, const int32_t* positions, const float* weights, const int32_t* counts,
                               const int32_t* offsets, unsigned char* grad_y, uint64_t ldd, float* grad_weights) {
     typedef typename V::elem_t E;
     constexpr int VEC = V::VEC;
-    if (blockIdx.x < pad_blocks) {
-        clear_padding<E>(blockIdx.x, counts, offsets, rows, grad_y, ldd, s.nvec, s.tail);
+    const uint32_t pads = pad_blocks(experts);
+    if (blockIdx.x < pads) {
+        clear_padding<E>(blockIdx.x, experts, counts, offsets, rows, grad_y, ldd, s.nvec, s.tail);
         return;
     }
     __shared__ float part[16][K];
     const uint32_t tid = threadIdx.x;
-    for (uint64_t t = blockIdx.x - pad_blocks; t < s.tokens; t += gridDim.x - pad_blocks) {
+    for (uint64_t t = blockIdx.x - pads; t < s.tokens; t += gridDim.x - pads) {
         const unsigned char* g = grad + t * ldg * sizeof(E);
         for (uint32_t j0 = 0; j0 < s.top_k; j0 += K) {
             const uint32_t k = s.top_k - j0 < (uint32_t)K ? s.top_k - j0 : (uint32_t)K;

@@ -225,6 +225,33 @@ def run_one_expert_twice_and_positions_outside(comp):
     assert not res.any()
 
 
+@pytest.mark.parametrize("experts", [1, 3, 4, 7])
+@pytest.mark.parametrize("variant", [0, 8])
+def test_an_odd_number_of_experts_reads_no_further_count(comp, variant, experts):
+    """counts and offsets are parts of larger arrays whose next words, taken for one more expert's, would clear every row."""
+    import torch
+    ids = np.arange(24).reshape(12, 2) % experts
+    pos, c, o = sort(comp, ids, experts, 4)
+    rows = int(o[-1])
+    counts, offsets = torch.full((experts + 2,), -rows, dtype=torch.int32, device="cuda"), torch.full((experts + 3,), rows, dtype=torch.int32, device="cuda")
+    counts[:experts], offsets[:experts + 1] = c, o
+    counts, offsets = counts[:experts], offsets[:experts + 1]
+    x = torch.arange(1, 13, device="cuda").float()[:, None].expand(12, 40).contiguous()
+    want = torch.zeros(rows, 40, device="cuda")
+    want[pos.long().reshape(-1)] = x.repeat_interleave(2, 0)
+    comp.set_param("variant", variant)
+    try:
+        for _ in range(2):
+            out, gy, gw = (torch.full(z, 9.0, device="cuda") for z in ((rows, 40), (rows, 40), (12, 2)))
+            comp.token_dispatch(x, pos, counts, offsets, out)
+            assert torch.equal(out, want)
+            comp.token_combine_backward(x, out, pos, None, counts, offsets, gy, gw)
+            assert torch.equal(gy, want)
+            assert torch.equal(gw[:, 0], 40 * x[:, 0] ** 2) and torch.equal(gw[:, 1], gw[:, 0])
+    finally:
+        comp.set_param("variant", 0)
+
+
 # the last: more tokens than the grid has blocks for them, whose blocks take a second one
 @pytest.mark.parametrize("tokens,k,experts,hidden,kind", [(6007, 6, 40, 1000, "bfloat16"), (70001, 1, 8, 257, "float32"), (70001, 1, 8, 4104, "bfloat16")])
 def test_many_runs_in_order_equal_token_by_token(comp, tokens, k, experts, hidden, kind):
