@@ -231,10 +231,9 @@ int mi_ccl_fusion_reduce_static(const size_t* counts, size_t k, int dtype, size_
 /* result[0] = |multiplier| * sqrt(sum of the squares of all gradients), result[1] = the factor that a clipped step
  * multiplies its gradients with: multiplier * min(1, max_norm / (result[0] + 1e-6)), or multiplier when max_norm <= 0.
  * multiplier: what the gradients are yet to be multiplied with (1 / peers after a sum, 1 / loss scale).  A norm that is not
- * finite (squares are fp32: an element from 1.8e19 up overflows, one below 1e-19 counts for less than it is) gives result[1] = NaN, which mi_ccl_fusion_adamw takes as
- * "no step".  result: two floats on the device.  workspace: mi_ccl_fusion_norm_workspace bytes of device memory, 8-byte
- * aligned, needed by this call alone (calls that may overlap take one each).  The sum has a fixed order: the same
- * gradients give the same bits. */
+ * finite gives result[1] = NaN, which mi_ccl_fusion_adamw takes as "no step".  Squares and their sum are fp64.  result: two
+ * floats on the device.  workspace: mi_ccl_fusion_norm_workspace bytes of device memory, 8-byte aligned, needed by this call
+ * alone (calls that may overlap take one each).  The sum has a fixed order: the same gradients give the same bits. */
 size_t mi_ccl_fusion_norm_workspace(const mi_ccl_fusion_plan* plan);
 int mi_ccl_fusion_norm(mi_ccl_fusion_plan* plan, const void* const* grads, const void* fusion_buf, double multiplier,
                        double max_norm, float* result, void* workspace, size_t workspace_bytes, void* stream);

@@ -27,8 +27,8 @@ constexpr uint32_t kAdamwTile = 4 * kAdamwBlock;        // its elements
 static_assert(kStateBlock == 64 * 4, "four elements of each lane of a wave are one 8-bit block");
 
 // ---- norm ---------------------------------------------------------------------------------------------------------------
-// Partial sums of one launch: three blocks per CU, each with the next item's address at hand.  800 M bf16 elements: 227 us
-// with 768 blocks (7.06 TB/s, what reading alone reaches), 250 with 512, 232 with 1,024, 246 with 2,048 to 16,384; 265 where
+// Partial sums of one launch: three blocks per CU, each with the next item's address at hand.  800 M bf16 elements: 226 us
+// with 768 blocks (7.07 TB/s, what reading alone reaches), 250 with 512, 232 with 1,024, 246 with 2,048 to 16,384; 265 where
 // the blocks look an item up when they come to it.
 constexpr uint32_t kNormBlocks = 768;
 
@@ -53,8 +53,8 @@ struct NormItem {
     }
 };
 
-// One double per block: squares are summed in fp32 over the at most 33 elements that a lane has of an item (16 KiB of one
-// tensor), everything above in fp64 and in a fixed order.
+// One double per block.  Squares and sums are fp64 throughout, in a fixed order: no finite gradient overflows or is lost, and
+// memory is still what bounds the kernel (226 us for 800 M bf16 elements, with squares in fp32 226 too).
 template <class V, bool BUFFER>
 __global__ void __launch_bounds__(kBlock)
 fusion_norm_kernel(FusionPtrs grads, const unsigned char* buffer, NormTables tb, double* partial) {
@@ -62,7 +62,7 @@ fusion_norm_kernel(FusionPtrs grads, const unsigned char* buffer, NormTables tb,
     constexpr uint32_t ES = sizeof(E), VEC = V::VEC;
     __shared__ double part[kBlock / 64];
     const uint32_t tid = threadIdx.x;
-    double sum = 0.0;
+    double sum[2] = { 0.0, 0.0 };
     NormItem<ES, BUFFER> next(grads, buffer, tb, blockIdx.x);
     for (uint32_t it = blockIdx.x; it < tb.nitems; it += gridDim.x) {
         const unsigned char* g = next.g;
@@ -70,7 +70,6 @@ fusion_norm_kernel(FusionPtrs grads, const unsigned char* buffer, NormTables tb,
         uint32_t head = fusion_head<ES>(g);
         if (head > nelem) head = nelem;
         const uint32_t nvec = (nelem - head) / VEC, tail = nelem - head - nvec * VEC;
-        float a = 0.0f;
         u32x4 x[4];
 #pragma unroll
         for (int u = 0; u < 4; u++)
@@ -83,12 +82,12 @@ fusion_norm_kernel(FusionPtrs grads, const unsigned char* buffer, NormTables tb,
             float f[VEC];
             V::widen(x[u], f);
 #pragma unroll
-            for (uint32_t i = 0; i < VEC; i++) a = __builtin_fmaf(f[i], f[i], a);
+            for (uint32_t i = 0; i < VEC; i++) sum[i % 2] = __builtin_fma((double)f[i], (double)f[i], sum[i % 2]);
         }
-        sum += (double)__builtin_fmaf(edge, edge, a);
+        sum[0] = __builtin_fma((double)edge, (double)edge, sum[0]);
     }
-    sum = wave_sum(sum);
-    if ((tid & 63u) == 0) part[tid >> 6] = sum;
+    sum[0] = wave_sum(sum[0] + sum[1]);
+    if ((tid & 63u) == 0) part[tid >> 6] = sum[0];
     __syncthreads();
     if (tid == 0) {
         double s = 0.0;
