@@ -38,15 +38,18 @@ bool words_aligned(const void* a, const void* b = nullptr, const void* c = nullp
     return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d | (uintptr_t)e) & 3u) == 0;
 }
 
-// How rows of `hidden` elements are shared out: U vectors per lane, as many waves per token as its row fills, and column
-// tiles of one row side by side in the grid when there are too few tokens to fill the chip.
+// How rows of `hidden` elements are shared out: U vectors per lane and one, two or four waves per column tile, the most that leave no
+// more lanes without a vector than one wave per tile does; a row's tiles are side by side in the grid.  combine, 16,384 tokens x
+// 8 rows of 10 KiB: 250 us in five tiles of 2 KiB, 320 in one of 8 KiB and a quarter of another; rows of 14 KiB 349 and 383.  Where there
+// are too few tokens to fill the chip, the most waves that a row fills (dispatch of 7 x 8 rows of 14 KiB 3.9 us, 4.3 in narrow tiles).
 RowShape row_shape(size_t hidden, int dtype, size_t n_tokens, int top_k, int u) {
     RowShape s;
     const uint32_t vec = 16 / (uint32_t)fusion_dtype_size(dtype);
     s.nvec = (uint32_t)(hidden / vec);
     s.tail = (uint32_t)(hidden % vec);
     s.log_waves = 0;
-    while (s.log_waves < 2 && (64u << s.log_waves) * u < s.nvec) s.log_waves++;
+    const uint32_t wave = 64u * u, tiles = (s.nvec + wave - 1) / wave;
+    while (s.log_waves < 2 && (n_tokens < 256 ? (1u << s.log_waves) < tiles : tiles && tiles % (2u << s.log_waves) == 0)) s.log_waves++;
     const uint32_t width = (64u << s.log_waves) * u;
     s.cols = s.nvec ? (s.nvec + width - 1) / width : 1;
     s.top_k = (uint32_t)top_k;
@@ -90,9 +93,12 @@ int sort_launch(const I* ids, uint32_t n, uint32_t experts, uint32_t align, uint
 }
 
 // Vectors of a row that a lane takes at once.  16,384 tokens x 8 rows of 8 KiB: dispatch 261 us with one, 264 with two, 278 with
-// four (a wave's stores go to eight places; more of them at once only mix more); combine 207, 203 and 205.
+// four (a wave's stores go to eight places; more of them at once only mix more); combine 207, 203 and 205.  Rows that one vector per lane
+// of a wave covers are combined with one (rows of 1 KiB: 31 us, 35 with two).
 constexpr int kDispatchU = 1;
-constexpr int kCombineU = 2;
+int combine_u(size_t hidden, int dtype) {
+    return hidden * fusion_dtype_size(dtype) <= 64 * 16 ? 1 : 2;
+}
 
 template <class E>
 void dispatch_launch(const RowShape& s, uint32_t experts, hipStream_t stream, const void* x, size_t ld_x, const int32_t* positions,
@@ -101,19 +107,26 @@ void dispatch_launch(const RowShape& s, uint32_t experts, hipStream_t stream, co
                        (const unsigned char*)x, (uint64_t)ld_x, s, experts, positions, counts, offsets, (unsigned char*)out, (uint64_t)ld_out, (uint64_t)rows);
 }
 
-template <class V, int K>
+template <class V, int U, int K>
 void combine_launch(const RowShape& s, hipStream_t stream, const void* y, size_t ld_y, size_t rows, const int32_t* positions,
                     const float* weights, void* out, size_t ld_out) {
-    hipLaunchKernelGGL((token_combine_kernel<V, kCombineU, K>), dim3(column_blocks(s), token_blocks(s)), dim3(kBlock), 0, stream, (const unsigned char*)y,
+    hipLaunchKernelGGL((token_combine_kernel<V, U, K>), dim3(column_blocks(s), token_blocks(s)), dim3(kBlock), 0, stream, (const unsigned char*)y,
                        (uint64_t)ld_y, (uint64_t)rows, s, positions, weights, (unsigned char*)out, (uint64_t)ld_out);
 }
-template <class V>
+template <class V, int U>
 void combine_by_k(const RowShape& s, hipStream_t stream, const void* y, size_t ld_y, size_t rows, const int32_t* positions,
                   const float* weights, void* out, size_t ld_out) {
-    if (s.top_k == 1) combine_launch<V, 1>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
-    else if (s.top_k == 2) combine_launch<V, 2>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
-    else if (s.top_k <= 4) combine_launch<V, 4>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
-    else combine_launch<V, 8>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    if (s.top_k == 1) combine_launch<V, U, 1>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    else if (s.top_k == 2) combine_launch<V, U, 2>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    else if (s.top_k <= 4) combine_launch<V, U, 4>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    else combine_launch<V, U, 8>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+}
+
+template <class V>
+void combine_by_u(const RowShape& s, int u, hipStream_t stream, const void* y, size_t ld_y, size_t rows, const int32_t* positions,
+                  const float* weights, void* out, size_t ld_out) {
+    if (u == 1) combine_by_k<V, 1>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
+    else combine_by_k<V, 2>(s, stream, y, ld_y, rows, positions, weights, out, ld_out);
 }
 
 struct BackwardArgs {
@@ -160,14 +173,17 @@ bool wants_order(int dtype, size_t n_tokens, int top_k, size_t hidden) {
         return false;
     return entries * hidden * fusion_dtype_size(dtype) >= kOrderBytes || mi_ccl_get_param("variant") == 8;
 }
-// Lanes of an entry, 64 to 512.  Dispatch takes no fewer than the row has vectors (one load and one store each); the gradient,
-// which has more to do per vector, lets a third of them go round twice.  26,296 tokens x 5 rows of 139 vectors: dispatch 76 us with 256
-// lanes, 83 with 128; gradient 158 with 128, 206 with 256.  65,536 x 1 rows of 230 vectors: gradient 132 with 256, 143 with 128.
-// Under 256 lanes a block of 256 takes several entries (26,296 x 8 rows of 64 vectors: dispatch 40 us, 51 in blocks of 64).
-uint32_t order_log_lanes(uint32_t nvec, bool one_each) {
-    uint32_t log_lanes = 6;
-    while (log_lanes < 9 && (one_each ? (1u << log_lanes) : (3u << log_lanes) / 2) < nvec) log_lanes++;
-    return log_lanes;
+// Lanes of an entry, whole waves, 64 to 512.  Dispatch has one load and one store per vector: as many lanes as the row has
+// vectors (16,384 tokens x 8 rows of 320 vectors: 112 us with 320 lanes, 133 with 512, 124 with 192 twice round; of 160 vectors 60 with
+// 192, 70 with 256).  The gradient, which has more to do per vector, takes a power of two and lets a third of the lanes go round twice:
+// 160 vectors 127 us with 128 lanes, 130 with 192; 320 vectors 234 with 256, 252 with 320; 26,296 x 5 rows of 139 vectors 158 with
+// 128, 206 with 256.  Up to 128 lanes a block of 256 takes several entries (26,296 x 8 rows of 64 vectors: dispatch 40 us, 51 in
+// blocks of 64).
+uint32_t order_lanes(uint32_t nvec, bool one_each) {
+    if (one_each) return nvec <= 64 ? 64u : nvec < 512 ? (nvec + 63) / 64 * 64 : 512u;
+    uint32_t lanes = 64;
+    while (lanes < 512 && lanes + lanes / 2 < nvec) lanes <<= 1;
+    return lanes;
 }
 // Entries per run: what keeps the run's tokens within 2 MiB, half of an XCD's L2, and leaves no XCD without a run in a tenth of the
 // turns (an XCD takes every eighth run).  Dispatch, two buffer sets in turn: 16,384 tokens x 8 of 8 KiB 184 us with 2,048 entries, 190 with
@@ -182,12 +198,10 @@ uint32_t order_log_run(uint64_t entries, uint32_t top_k, uint64_t row_bytes) {
     }
     return log_run;
 }
-uint32_t order_block(uint32_t log_lanes) {
-    return log_lanes < 8 ? 256u : 1u << log_lanes;
-}
-uint32_t order_blocks(uint64_t entries, uint32_t log_run, uint32_t log_lanes) {         // eight runs at a time
+constexpr uint32_t kOrderMulti = 128;        // lanes of an entry up to which a block takes several (64 or 128: powers of two)
+uint32_t order_blocks(uint64_t entries, uint32_t log_run, uint32_t lanes) {         // eight runs at a time
     const uint64_t runs = (entries + (1u << log_run) - 1) >> log_run;
-    return (uint32_t)((((runs + 7) / 8 * 8) << log_run) / (order_block(log_lanes) >> log_lanes));
+    return (uint32_t)((((runs + 7) / 8 * 8) << log_run) / (lanes <= kOrderMulti ? kOrderedMultiBlock / lanes : 1));
 }
 int order_launch(const int32_t* positions, uint64_t entries, uint32_t log_run, size_t rows, OrderedEntry* order, hipStream_t stream) {
     uint32_t shift = 0;
@@ -200,10 +214,14 @@ int order_launch(const int32_t* positions, uint64_t entries, uint32_t log_run, s
 struct OrderedArgs {
     dim3 grid, block;
     hipStream_t stream;
-    uint32_t experts, log_lanes, log_run;
+    uint32_t experts, log_lanes, log_run;       // log_lanes: of several entries per block
     uint64_t entries;
     const OrderedEntry* order;
-    bool multi() const { return log_lanes < 8; }
+    bool multi;
+    OrderedArgs(uint32_t lanes, uint32_t experts_, uint32_t log_run_, uint64_t entries_, const OrderedEntry* order_, hipStream_t stream_)
+        : grid(pad_blocks(experts_) + order_blocks(entries_, log_run_, lanes)), block(lanes <= kOrderMulti ? kOrderedMultiBlock : lanes),
+          stream(stream_), experts(experts_), log_lanes(lanes == 64 ? 6 : 7), log_run(log_run_), entries(entries_), order(order_),
+          multi(lanes <= kOrderMulti) {}
 };
 template <class E, bool MULTI>
 void dispatch_ordered_launch(const OrderedArgs& o, const RowShape& s, const void* x, size_t ld_x, const int32_t* counts, const int32_t* offsets,
@@ -215,7 +233,7 @@ void dispatch_ordered_launch(const OrderedArgs& o, const RowShape& s, const void
 template <class E>
 void dispatch_ordered(const OrderedArgs& o, const RowShape& s, const void* x, size_t ld_x, const int32_t* counts, const int32_t* offsets, void* out,
                       size_t ld_out, size_t rows) {
-    if (o.multi()) dispatch_ordered_launch<E, true>(o, s, x, ld_x, counts, offsets, out, ld_out, rows);
+    if (o.multi) dispatch_ordered_launch<E, true>(o, s, x, ld_x, counts, offsets, out, ld_out, rows);
     else dispatch_ordered_launch<E, false>(o, s, x, ld_x, counts, offsets, out, ld_out, rows);
 }
 
@@ -228,10 +246,8 @@ void backward_ordered_launch(const OrderedArgs& o, const BackwardArgs& a) {
 template <class V, bool DOT>
 void backward_ordered(const BackwardArgs& a, const OrderedEntry* order, uint32_t log_run) {
     const uint64_t entries = a.s.tokens * a.s.top_k;
-    const uint32_t log_lanes = order_log_lanes(a.s.nvec, false);
-    const OrderedArgs o = { dim3(pad_blocks(a.experts) + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), a.stream, a.experts,
-                            log_lanes, log_run, entries, order };
-    if (o.multi()) backward_ordered_launch<V, DOT, true>(o, a);
+    const OrderedArgs o(order_lanes(a.s.nvec, false), a.experts, log_run, entries, order, a.stream);
+    if (o.multi) backward_ordered_launch<V, DOT, true>(o, a);
     else backward_ordered_launch<V, DOT, false>(o, a);
 }
 template <class V>
@@ -310,9 +326,7 @@ int mi_ccl_token_dispatch(int dtype, const void* x, size_t ld_x, size_t n_tokens
         const int rc = order_launch(positions, entries, log_run, out_rows, order, (hipStream_t)stream);
         if (rc != MI_CCL_SUCCESS)
             return rc;
-        const uint32_t experts = (uint32_t)n_experts, log_lanes = order_log_lanes(s.nvec, true);
-        const OrderedArgs o = { dim3(pad_blocks(experts) + order_blocks(entries, log_run, log_lanes)), dim3(order_block(log_lanes)), (hipStream_t)stream,
-                                experts, log_lanes, log_run, entries, order };
+        const OrderedArgs o(order_lanes(s.nvec, true), (uint32_t)n_experts, log_run, entries, order, (hipStream_t)stream);
         if (fusion_dtype_size(dtype) == 4) dispatch_ordered<uint32_t>(o, s, x, ld_x, counts, offsets, out, ld_out, out_rows);
         else dispatch_ordered<uint16_t>(o, s, x, ld_x, counts, offsets, out, ld_out, out_rows);
         return launched("token_dispatch_ordered_kernel");
@@ -333,10 +347,11 @@ int mi_ccl_token_combine(int dtype, const void* y, size_t ld_y, size_t y_rows, c
     if ((y_rows && !row_pointer_ok(y, dtype)) || !row_pointer_ok(out, dtype) || !positions || ld_y < hidden || ld_out < hidden ||
         hidden > kMaxRows || n_tokens > kMaxRows / (uint64_t)top_k || y_rows > kMaxRows || !words_aligned(positions, weights))
         return MI_CCL_INVALID_ARGUMENTS;
-    const RowShape s = row_shape(hidden, dtype, n_tokens, top_k, kCombineU);
-    if (dtype == MI_CCL_FLOAT32) combine_by_k<F32Vec>(s, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
-    else if (dtype == MI_CCL_BFLOAT16) combine_by_k<Bf16Vec>(s, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
-    else combine_by_k<Fp16Vec>(s, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
+    const int u = combine_u(hidden, dtype);
+    const RowShape s = row_shape(hidden, dtype, n_tokens, top_k, u);
+    if (dtype == MI_CCL_FLOAT32) combine_by_u<F32Vec>(s, u, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
+    else if (dtype == MI_CCL_BFLOAT16) combine_by_u<Bf16Vec>(s, u, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
+    else combine_by_u<Fp16Vec>(s, u, (hipStream_t)stream, y, ld_y, y_rows, positions, weights, out, ld_out);
     return launched("token_combine_kernel");
 }
 

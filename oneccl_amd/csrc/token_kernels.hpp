@@ -276,6 +276,7 @@ token_order_kernel(const int32_t* positions, uint64_t n, uint32_t run, uint64_t 
 // entry is on the scalar unit (as the lanes' own values it cost a tenth).  Entries come run after run, eight runs side by
 // side, one per XCD (blocks go round the XCDs by their index).
 constexpr int kOrderedBlock = 512;         // lanes at most
+constexpr uint32_t kOrderedMultiBlock = 256;
 template <bool MULTI>
 struct OrderedLane {
     uint64_t at;                // the group's place in the order
@@ -284,7 +285,7 @@ struct OrderedLane {
         lanes = MULTI ? 1u << log_lanes : blockDim.x;
         lane = MULTI ? threadIdx.x & (lanes - 1) : threadIdx.x;
         const uint32_t xcd = block & 7u;
-        const uint32_t r = MULTI ? (block >> 3) * (blockDim.x >> log_lanes) + __builtin_amdgcn_readfirstlane(threadIdx.x >> log_lanes) : block >> 3;
+        const uint32_t r = MULTI ? (block >> 3) * (kOrderedMultiBlock >> log_lanes) + __builtin_amdgcn_readfirstlane(threadIdx.x >> log_lanes) : block >> 3;
         at = ((((uint64_t)(r >> log_run) << 3) + xcd) << log_run) + (r & ((1u << log_run) - 1));
     }
 };

@@ -252,8 +252,10 @@ def test_an_odd_number_of_experts_reads_no_further_count(comp, variant, experts)
         comp.set_param("variant", 0)
 
 
-# the last: more tokens than the grid has blocks for them, whose blocks take a second one
-@pytest.mark.parametrize("tokens,k,experts,hidden,kind", [(6007, 6, 40, 1000, "bfloat16"), (70001, 1, 8, 257, "float32"), (70001, 1, 8, 4104, "bfloat16")])
+# 70,001 x 4104: more tokens than the grid has blocks for them, whose blocks take a second one; 192, 384 and 512 lanes per row, several column
+# tiles per row
+@pytest.mark.parametrize("tokens,k,experts,hidden,kind", [(6007, 6, 40, 1000, "bfloat16"), (70001, 1, 8, 257, "float32"), (70001, 1, 8, 4104, "bfloat16"),
+                                                             (5003, 7, 13, 1540, "bfloat16"), (9001, 1, 5, 5124, "float16"), (7001, 1, 5, 2565, "float32")])
 def test_many_runs_in_order_equal_token_by_token(comp, tokens, k, experts, hidden, kind):
     """From 64 MiB of rows the order is taken by itself (runs on every XCD, a last run that is not full): the same rows as without
     scratch memory, to the bit; the weights' gradients within the bound of their sums."""
