@@ -154,20 +154,22 @@ def _stream(stream):
     return stream.cuda_stream
 
 
+_native = None              # oneccl_amd._tensors, loaded behind torch, whose libraries it needs; False where it was not built
+
+
 def _device():
+    global _native
     import torch
+    if _native is None:
+        try:
+            from . import _tensors as _native
+        except ImportError:
+            _native = False
     return torch.cuda.current_device()
 
 
 def _ptr_array(xs):
     return (C.c_void_p * len(xs))(*[_ptr(x) for x in xs])
-
-
-def _addresses(tensors):
-    """_ptr_array of what is known to be tensors, as an array whose buffer_info()[0] is the table's address (built a third
-    faster)."""
-    import torch
-    return array.array("Q", list(map(torch.Tensor.data_ptr, tensors)))
 
 
 _TORCH_DTYPE = {INT32: "int32", INT64: "int64", FLOAT16: "float16", FLOAT32: "float32", BFLOAT16: "bfloat16"}
@@ -191,6 +193,10 @@ def _refuse(what, t, wanted):
 
 def _memory(what, t, dtype, least, here):
     """Address of a contiguous tensor of the current GPU with at least `least` elements."""
+    if _native:
+        address = _native.memory(t, dtype, least, here)
+        if address is not None:
+            return address
     if t is None or t.dtype is not dtype or t.numel() < least or t.get_device() != here or not t.is_contiguous():
         _refuse(what, t, f"contiguous {dtype}, {least} elements at least, on cuda:{here}")
     return t.data_ptr()
@@ -219,10 +225,14 @@ def _workspace(workspace, need, here, stream):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
-def _check_tensors(what, tensors, dtype, least, here):
-    """_memory's conditions for a list, least[i] elements of the i-th.  A step over hundreds of tensors comes through here, hence
-    one C-level pass per property."""
+def _table(what, tensors, dtype, least, here):
+    """(what ctypes takes as the address of a table of the tensors' addresses, what holds it): _memory's conditions for a list, least[i]
+    elements of the i-th (an array of 64-bit numbers)."""
     import torch
+    if _native:
+        table = _native.addresses(tensors, dtype, least, here)
+        if table is not None:
+            return table, table
     T = torch.Tensor
     try:
         devices, kinds = set(map(T.get_device, tensors)), {t.dtype for t in tensors}
@@ -235,8 +245,10 @@ def _check_tensors(what, tensors, dtype, least, here):
         raise ValueError(f"{what}: not contiguous")
     if kinds != {dtype}:
         raise ValueError(f"{what}: {kinds}, {dtype} is wanted")
-    if sizes != least and any(map(operator.lt, sizes, least)):
+    if any(map(operator.lt, sizes, least)):
         raise ValueError(f"{what}: a tensor has fewer elements than the plan says")
+    table = array.array("Q", list(map(T.data_ptr, tensors)))
+    return table.buffer_info()[0], table
 
 
 def datatype_size(dtype):
@@ -376,6 +388,9 @@ class FusionPlan:
         self.k = k
         self.dtype = dtype
         self.counts = [int(c) for c in counts]
+        self._least = array.array("q", self.counts)
+        import torch
+        self._torch_dtype = getattr(torch, _TORCH_DTYPE.get(dtype, "float32"))
         self.norm_workspace = lib().mi_ccl_fusion_norm_workspace(h)       # bytes
         self._here = _device()              # the GPU that holds the plan's table
         self.elements = lib().mi_ccl_fusion_plan_elements(h)      # of a state or fp32 copy of the weights in the plan's layout
@@ -414,14 +429,12 @@ class FusionPlan:
 
     def _gradients(self, grads, here):
         """(address of a table of addresses, address of a fusion buffer, what has to live until the call has returned)."""
-        import torch
-        kind = getattr(torch, _TORCH_DTYPE.get(self.dtype, "float32"))
+        kind = self._torch_dtype
         if isinstance(grads, (list, tuple)):
             if len(grads) != self.k:
                 raise ValueError("the gradients are not the plan's tensors")
-            _check_tensors("gradients", grads, kind, self.counts, here)
-            table = _addresses(grads)
-            return table.buffer_info()[0], None, table
+            address, table = _table("gradients", grads, kind, self._least, here)
+            return address, None, table
         return None, _memory("gradients", grads, kind, self.elements, here), None
 
     def norm(self, grads, result, multiplier=1.0, max_norm=0.0, workspace=None, stream=None):
@@ -430,7 +443,7 @@ class FusionPlan:
         import torch
         here = self._device()
         res = _memory("result", result, torch.float32, 2, here)
-        lst, buf, _table = self._gradients(grads, here)
+        lst, buf, _held = self._gradients(grads, here)
         ws, size, _keep = _workspace(workspace, self.norm_workspace, here, stream)
         _check(lib().mi_ccl_fusion_norm(self._h, lst, buf, multiplier, max_norm, res, ws, size, _stream(stream)), "mi_ccl_fusion_norm")
 
@@ -444,7 +457,7 @@ class FusionPlan:
         here = self._device()
         if len(params) != self.k or params[0] is None:
             raise ValueError("the parameters are not the plan's tensors")
-        _check_tensors("params", params, params[0].dtype, self.counts, here)
+        weights, _held_too = _table("params", params, params[0].dtype, self._least, here)
         eight = exp_avg.dtype is torch.uint8
         kind = torch.uint8 if eight else torch.float32
         m, v = _memory("exp_avg", exp_avg, kind, self.elements, here), _memory("exp_avg_sq", exp_avg_sq, kind, self.elements, here)
@@ -455,9 +468,8 @@ class FusionPlan:
         o = AdamwOptions(lr, beta1, beta2, eps, weight_decay, int(step), 0 if seed is None else int(seed), int(seed is not None),
                          _optional("step_ptr", step_ptr, torch.int64, 1, here), _optional("lr_ptr", lr_ptr, torch.float32, 1, here),
                          _optional("grad_scale", grad_scale, torch.float32, 1, here), ws)
-        lst, buf, _table = self._gradients(grads, here)
-        table = _addresses(params)
-        _check(lib().mi_ccl_fusion_adamw(self._h, _kind(params[0]), table.buffer_info()[0], lst, buf, STATE_8BIT if eight else STATE_FP32,
+        lst, buf, _held = self._gradients(grads, here)
+        _check(lib().mi_ccl_fusion_adamw(self._h, _kind(params[0]), weights, lst, buf, STATE_8BIT if eight else STATE_FP32,
                                          m, v, sc, _optional("master", master, torch.float32, self.elements, here), C.byref(o),
                                          _stream(stream)), "mi_ccl_fusion_adamw")
 
@@ -507,6 +519,10 @@ def fusion_reduce_static(counts, dtype, align, op, own_tensors, peers, out_tenso
 
 def _rows(what, t, hidden, dtype, here):
     """(rows, elements from row to row, address) of a matrix whose rows are contiguous and do not overlap."""
+    if _native:
+        found = _native.rows(t, hidden, dtype, here)
+        if found is not None:
+            return found
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[1] != hidden or t.dtype is not dtype or t.get_device() != here or (hidden > 1 and stride[1] != 1) or \
             (shape[0] > 1 and stride[0] < hidden):

@@ -94,3 +94,75 @@ def test_optimizer_calls_refuse_a_missing_plan():
     assert L.mi_ccl_fusion_state_decode(None, A, A, A, c.FLOAT32, A, A, None) == BAD
     assert L.mi_ccl_fusion_state_encode(None, c.FLOAT32, A, A, A, A, A, None) == BAD
     assert L.mi_ccl_fusion_norm_workspace(None) == 0 and L.mi_ccl_fusion_plan_elements(None) == 0
+
+
+# ---- what the binding asks of tensors in one pass; device -1 is host memory
+
+def tensors():
+    return pytest.importorskip("oneccl_amd._tensors", reason="not built")
+
+
+def test_memory_of_a_tensor():
+    import torch
+    t = tensors()
+    x = torch.zeros(4, 6)
+    assert t.memory(x, torch.float32, 24, -1) == x.data_ptr()
+    assert t.memory(torch.nn.Parameter(x), torch.float32, 0, -1) == x.data_ptr()
+    assert t.memory(x[1], torch.float32, 6, -1) == x.data_ptr() + 24
+    assert t.memory(torch.zeros(0), torch.float32, 0, -1) == 0
+    for bad in (None, 3, [x], x.t(), x[:, 1:], x.double(), x.to("meta"), x.to_sparse(), torch.zeros(23), x.expand(2, 4, 6)):
+        assert t.memory(bad, torch.float32, 24, -1) is None
+    for call in ((x, "float32", 24, -1), (x, None, 24, -1), (x, torch.float32, 24, 0), (x, torch.float32, None, -1), (x, torch.float32, 1 << 70, -1),
+                 (x, torch.float32, 24, 1.5), (x, torch.float32, 24), ()):
+        assert t.memory(*call) is None
+
+
+def test_rows_of_a_matrix():
+    import torch
+    t = tensors()
+    x = torch.zeros(4, 6)
+    assert t.rows(x, 6, torch.float32, -1) == (4, 6, x.data_ptr())
+    assert t.rows(x[::2, 1:5], 4, torch.float32, -1) == (2, 12, x.data_ptr() + 4)
+    assert t.rows(x[1:2], 6, torch.float32, -1) == (1, 6, x.data_ptr() + 24)
+    assert t.rows(x[:0], 6, torch.float32, -1)[:2] == (0, 6)
+    assert t.rows(x[:, :1], 1, torch.float32, -1) == (4, 6, x.data_ptr())
+    assert t.rows(x[:, :0], 0, torch.float32, -1)[:2] == (4, 6)
+    for bad, hidden in ((x, 5), (x[0], 6), (x.t(), 4), (x[:1].expand(4, 6), 6), (x[:, ::2], 3), (x.half(), 6), (x[None], 6), (None, 6), (x.to("meta"), 6)):
+        got = t.rows(bad, hidden, torch.float32, -1)
+        assert got is None
+
+
+def test_addresses_of_tensors():
+    import array
+    import torch
+    t = tensors()
+    xs = [torch.zeros(n) for n in (3, 0, 5, 1)]
+    least = array.array("q", [3, 0, 5, 1])
+    for seq in (xs, tuple(xs)):
+        assert array.array("Q", t.addresses(seq, torch.float32, least, -1)).tolist() == [x.data_ptr() for x in xs]
+    assert t.addresses([], torch.float32, array.array("q"), -1) == b""
+    for bad in (xs[:3], xs + xs[:1], [None] + xs[1:], [x.double() for x in xs], xs[::-1], iter(xs), None, xs[:3] + [3]):
+        assert t.addresses(bad, torch.float32, least, -1) is None
+    assert t.addresses(xs, torch.float32, least, 0) is None
+    assert t.addresses(xs, torch.float32, [3, 0, 5, 1], -1) is None
+    assert t.addresses(xs[:3] + [torch.zeros(4, 3).t()], torch.float32, least, -1) is None
+
+
+def test_the_binding_refuses_the_same_without_the_native_pass(monkeypatch):
+    import array
+    import torch
+    t = tensors()
+    x = torch.zeros(4, 6)
+    for native in (t, False):
+        monkeypatch.setattr(c, "_native", native)
+        assert c._memory("x", x, torch.float32, 24, -1) == x.data_ptr()
+        assert c._rows("x", x, 6, torch.float32, -1) == (4, 6, x.data_ptr())
+        address, table = c._table("x", [x, x[1]], torch.float32, array.array("q", [24, 6]), -1)
+        assert array.array("Q", table).tolist() == [x.data_ptr(), x[1].data_ptr()]
+        for call in (lambda: c._memory("x", x.t(), torch.float32, 24, -1), lambda: c._memory("x", None, torch.float32, 0, -1),
+                     lambda: c._rows("x", x, 5, torch.float32, -1), lambda: c._table("x", [x, None], torch.float32, array.array("q", [1, 1]), -1),
+                     lambda: c._table("x", [x], torch.float32, array.array("q", [25]), -1),
+                     lambda: c._table("x", [x], torch.float16, array.array("q", [1]), -1),
+                     lambda: c._table("x", [x], torch.float32, array.array("q", [1]), 0)):
+            with pytest.raises(ValueError):
+                call()
