@@ -5,6 +5,7 @@ there is no CPU fallback: a missing library raises at load time.
 """
 import array
 import ctypes as C
+import functools
 import operator
 import os
 
@@ -538,6 +539,8 @@ def token_rows(n_tokens, top_k, n_experts, align=1, capacity=0):
     return r.value
 
 
+# both are arithmetic on the sizes, looked up by them: a step asks for the same ones again and again, at 1.2 us each
+@functools.lru_cache(maxsize=1024)
 def token_sort_workspace(n_tokens, top_k, n_experts):
     r = C.c_size_t()
     _check(lib().mi_ccl_token_sort_workspace(n_tokens, top_k, n_experts, C.byref(r)), "mi_ccl_token_sort_workspace")
@@ -562,6 +565,7 @@ def token_sort(expert_ids, n_experts, positions, counts, offsets, align=1, capac
            "mi_ccl_token_sort")
 
 
+@functools.lru_cache(maxsize=1024)
 def token_order_workspace(dtype, n_tokens, top_k, hidden):
     """Bytes of scratch memory that a large token_dispatch or token_combine_backward goes faster with."""
     r = C.c_size_t()
@@ -661,6 +665,7 @@ def last_kernel():
 
 def set_param(name, value):
     _check(lib().mi_ccl_set_param(name.encode(), int(value)), f"mi_ccl_set_param({name})")
+    token_order_workspace.cache_clear()         # "variant" is in it
 
 
 def get_param(name):
