@@ -492,3 +492,47 @@ def test_refusals(comp):
         bad = list(args)
         bad[i] = x
         assert L.mi_ccl_fusion_adamw(*bad) == comp.INVALID_ARGUMENTS, i
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_offsets_past_32_bits(comp, eight):
+    """A group of 2^31 elements and more: bytes of gradients, weights and states past 2^32.  All is zero but pieces at the ends and around
+    the elements where a 32-bit offset of bytes or elements would turn over."""
+    import torch
+    counts = [70001, (1 << 31) + 12345, 4099]
+    plan = comp.FusionPlan(counts, comp.BFLOAT16, 2 * BLOCK if eight else 2)
+    first, n = [plan.offset(i) // 2 for i in range(3)], plan.elements
+    buffer = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    params = [torch.zeros(c, dtype=torch.bfloat16, device="cuda") for c in counts]
+    states = [torch.zeros(n, dtype=torch.uint8 if eight else torch.float32, device="cuda") for _ in range(2)]
+    scales = torch.zeros(2 * -(-n // BLOCK), dtype=torch.uint8, device="cuda") if eight else None
+    gen = torch.Generator("cuda").manual_seed(5)
+    pieces = [(0, 0, 5000), (1, 0, 700), (1, (1 << 30) - 777, 1500), (1, (1 << 31) - first[1] - 600, 1111), (1, counts[1] - 800, 800), (2, 0, 4099)]
+    for t, e, size in pieces:
+        buffer[first[t] + e:first[t] + e + size] = (1e-3 * torch.randn(size, device="cuda", generator=gen)).bfloat16()
+        params[t][e:e + size] = (0.02 * torch.randn(size, device="cuda", generator=gen)).bfloat16()
+    old = [params[t][e:e + size].double().cpu().numpy() for t, e, size in pieces]
+    grads = [buffer[first[t] + e:first[t] + e + size].double().cpu().numpy() for t, e, size in pieces]
+    exact = math.sqrt(sum(float((g ** 2).sum()) for g in grads))
+    result = torch.zeros(2, device="cuda")
+    for source in (buffer, [buffer[f:f + c] for f, c in zip(first, counts)]):
+        plan.norm(source, result)
+        assert abs(result[0].item() - exact) <= 1.01 * U * exact
+    plan.adamw(params, buffer, *states, scales=scales, **HYPER)
+    nonzero = sum(int(torch.count_nonzero(p[a:a + (1 << 28)])) for p in params for a in range(0, p.numel(), 1 << 28))
+    assert 0 < nonzero <= sum(size for _, _, size in pieces)
+    for (t, e, size), w, g in zip(pieces, old, grads):
+        x, m, v, dx, dm, dv = adamw(w, 0 * w, 0 * w, g, **HYPER)
+        got = params[t][e:e + size].double().cpu().numpy()
+        assert (np.abs(got - x) <= dx + half_step("bfloat16", np.abs(x) + dx)).all()
+        at = slice(first[t] + e, first[t] + e + size)
+        if not eight:
+            assert (np.abs(states[0][at].double().cpu().numpy() - m) <= dm).all()
+            assert (np.abs(states[1][at].double().cpu().numpy() - v) <= dv).all()
+        else:
+            assert int(torch.count_nonzero(states[1][at])) == np.count_nonzero(g)       # a second moment above zero stays above it
+
+
+def test_the_native_pass_over_tensors_is_built(comp):
+    comp.FusionPlan([3], comp.FLOAT32, 1)
+    assert comp._native

@@ -372,3 +372,34 @@ def test_refusals_of_the_binding(comp):
                  lambda: comp.token_combine(torch.zeros(1, 8, device="cuda").expand(3, 8), pos, None, torch.zeros(2, 8, device="cuda"))):
         with pytest.raises((ValueError, comp.CclError)):
             call()
+
+
+def test_rows_past_32_bits_of_bytes(comp):
+    """270,001 rows of 16 KiB: copies and products by one, to the bit, in both forms."""
+    import torch
+    tokens, hidden, experts = 270001, 8192, 4
+    rng = np.random.default_rng(3)
+    pos, counts, offsets = sort(comp, make_ids(rng, tokens, 1, experts), experts, 16)
+    rows = comp.token_rows(tokens, 1, experts, 16)
+    x = torch.randn(1, hidden, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).bfloat16().repeat(tokens, 1)
+    x[:, 0] = torch.arange(tokens, device="cuda").bfloat16()
+    x[:, 1] = (torch.arange(tokens, device="cuda") % 251).bfloat16()
+    x[:, hidden - 1] = (torch.arange(tokens, device="cuda") % 241).bfloat16()
+    none = torch.zeros(1, dtype=torch.int64, device="cuda")
+    out, back = torch.empty(rows, hidden, device="cuda", dtype=torch.bfloat16), torch.empty_like(x)
+    ones = torch.ones(tokens, 1, device="cuda")
+    assert out.numel() * 2 > 1 << 32
+    for ws in (None, none):
+        for call in (lambda: comp.token_dispatch(x, pos, counts, offsets, out, workspace=ws),
+                     lambda: comp.token_combine_backward(x, None, pos, ones, counts, offsets, out, workspace=ws)):
+            out.fill_(3.0)
+            call()
+            back.zero_()
+            comp.token_combine(out, pos, ones, back)
+            for t0 in range(0, tokens, 1 << 15):
+                part = slice(t0, t0 + (1 << 15))
+                assert torch.equal(out[pos[part, 0].long()], x[part]) and torch.equal(back[part], x[part])
+            end, begin = int(offsets[-1]), offsets[:-1] + counts
+            for e in range(experts):
+                assert not out[int(begin[e]):int(offsets[e + 1])].any()
+            assert (out[end:] == 3).all()
